@@ -102,7 +102,8 @@ void hipdec_destroy(hipdec_model *m);
  * pays the weights once with this.) */
 int hipdec_create_shared(const hipdec_model *base, uint32_t kv_dtype, uint32_t flags, hipdec_model **out);
 
-/* Text of the last error on this model (or of the last failed hipdec_create when m is NULL). */
+/* Text of the last error on this model (or, when m is NULL, of the last failed call without a model on the
+ * calling thread, hipdec_create among them). */
 const char *hipdec_last_error(const hipdec_model *m);
 
 /* Model::len / Model::set_len, lib.rs:209-215 (set_len clamps to cfg.seq). */
@@ -275,6 +276,131 @@ int hipdec_create_packed(const hipdec_config *cfg, const hipdec_packed_layer *la
 int hipdec_sample_fullvocab_noalloc(const float *d_logits, size_t vocab, const float *d_maxes, const float *d_sums,
                                     float temperature, float softcap, uint64_t *d_rng_state, uint32_t *d_out_token,
                                     void *stream);
+/* ---- operators on the caller's device buffers: a paged key-value cache, and drafted tokens ----
+ *
+ * No counterpart in the reference, whose cache is one contiguous window per model and which decodes one
+ * token at a time.  They are for programs that keep requests of their own: every d_ pointer is DEVICE
+ * memory of the current device, the kernels are enqueued on `stream` (a hipStream_t of the current device,
+ * NULL = its default stream) without waiting for them, nothing is allocated and nothing is kept between
+ * calls, so a call can be recorded into a graph.  Workspaces are the caller's: one per call in flight (two
+ * streams, or two graphs that may run at once, need one each).  Structs are read before the call returns.
+ * Errors are reported through hipdec_last_error(NULL) on the calling thread; after an error nothing was
+ * enqueued.  Numbers in device memory cannot be checked on the host: what each call makes of those that are
+ * out of range is said with it, and none leads outside the buffers described. */
+
+typedef enum {               /* number format of rows and logits */
+    HIPDEC_ROWS_F32 = 0,
+    HIPDEC_ROWS_BF16 = 1
+} hipdec_row_dtype;
+
+/* A pool of pages for keys and values, and the page table of its sequences: slot s of sequence q is slot
+ * s % page_size of page page_table[q * max_pages + s / page_size].  Element d of head h of a page's slot s
+ * lies at k[page * stride_page + s * stride_slot + h * stride_head + d], strides in elements; k and v share
+ * the strides.  A page may stand in several sequences (a shared prefix).  page_size: a power of two, at most
+ * 65536; strides: not negative, and no two elements of the pool in one place. */
+typedef struct {
+    void *k, *v;             /* device memory, hipdec_kv_dtype numbers */
+    uint32_t kv_dtype, page_size, n_pages, kv_heads, hd;
+    uint32_t n_seqs, max_pages;
+    const int32_t *page_table;   /* device memory [n_seqs][max_pages]; an entry outside 0 .. n_pages - 1: no page */
+    int64_t stride_page, stride_slot, stride_head;
+} hipdec_paged_cache;
+
+/* How rows are turned to their positions: pair i of the first rot_dim elements of a head by the angle
+ * position * d_freq[i], both results times `magnitude`.  interleaved: pair i is elements (2i, 2i + 1), as in
+ * the models of this library; otherwise elements (i, i + rot_dim / 2).  rot_dim: even, 0 .. hd. */
+typedef struct {
+    const double *d_freq;    /* device memory [rot_dim / 2] */
+    uint32_t rot_dim, interleaved;
+    float magnitude;
+} hipdec_rope;
+
+/* Angles per position (host memory, freq[rot_dim / 2]) and *magnitude for models whose context is `factor`
+ * times the `trained` positions they were trained on (theta: 10000 in the models of this library):
+ *   HIPDEC_ROPE_PLAIN   theta^(-2i / rot_dim)
+ *   HIPDEC_ROPE_LINEAR  the same divided by factor
+ *   HIPDEC_ROPE_BASE    theta replaced by theta * factor^(rot_dim / (rot_dim - 2)): the slowest pair is divided by
+ *                       factor, the fastest stays
+ *   HIPDEC_ROPE_PARTS   pairs that make at least `fast_turns` turns within `trained` positions stay, those that make
+ *                       at most `slow_turns` are divided by factor, those between are mixed in proportion;
+ *                       *magnitude = 0.1 ln(factor) + 1
+ * Needs no GPU.  rot_dim even and > 0, theta > 1, factor >= 1, trained > 0, fast_turns > slow_turns >= 0. */
+typedef enum {
+    HIPDEC_ROPE_PLAIN = 0, HIPDEC_ROPE_LINEAR = 1, HIPDEC_ROPE_BASE = 2, HIPDEC_ROPE_PARTS = 3
+} hipdec_rope_scaling;
+int hipdec_rope_frequencies(uint32_t scaling, uint32_t rot_dim, double theta, double factor, double trained,
+                            double slow_turns, double fast_turns, double *freq, float *magnitude);
+
+/* New rows of queries, keys and values (d_q: heads x hd elements of dtype, d_k / d_v: kv_heads x hd, row t at
+ * t * stride elements): queries are turned to d_positions[t] and written to d_q_out, keys are turned, and keys
+ * and values written to slot d_slots[t] of sequence d_seqs[t], rounded to the cache's format.  d_slots NULL:
+ * the position is the slot; d_seqs NULL: row t is of sequence t.  d_q_out may be d_q (with the same stride),
+ * otherwise no input and output overlap.  A row whose slot is negative (padding), or whose slot, sequence or
+ * page does not exist, writes no keys and values; its queries are turned all the same.  If two rows name one
+ * slot, either's numbers may stand in each of its elements. */
+typedef struct {
+    const void *d_q, *d_k, *d_v;
+    void *d_q_out;
+    uint32_t dtype, heads;               /* hipdec_row_dtype */
+    uint64_t n_rows;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const int32_t *d_positions, *d_slots, *d_seqs;
+} hipdec_new_rows;
+int hipdec_rope_append_paged(const hipdec_rope *rope, const hipdec_paged_cache *cache, const hipdec_new_rows *rows,
+                             void *stream);
+
+/* Attention of new tokens: row r has one query per head (d_q, heads x hd) and sees slots 0 .. d_lens[r] - 1 of
+ * sequence d_seqs[r] (NULL: sequence r); query heads h * g .. h * g + g - 1 read key head h, g = heads / kv_heads;
+ * d_out[r][h] = sum_s w_s v_s, w = softmax_s(scale * q . k_s), in the rows' format.  Several rows may be of one
+ * sequence with lengths of their own (the rows of a draft).  max_len bounds the lengths from the host's side:
+ * lengths above it, or above the page table's max_pages * page_size, count as that bound, those below zero as 0.
+ * A row without a slot (length 0, a sequence that does not exist) gives zeros; slots whose page does not
+ * exist are left out.  scale > 0.  hd: 64, 128, 192 or 256 (else HIPDEC_ERR_UNSUPPORTED); d_q, d_out and the
+ * cache 16-byte aligned with strides that are multiples of 16 bytes.  d_workspace: at least
+ * hipdec_attention_paged_workspace bytes for the same sizes and max_len, 16-byte aligned (may be NULL if that is 0). */
+typedef struct {
+    const void *d_q;
+    void *d_out;
+    uint32_t dtype, heads;               /* hipdec_row_dtype */
+    uint64_t n_rows;
+    int64_t q_stride, out_stride;        /* elements between rows */
+    const int32_t *d_lens, *d_seqs;
+    uint64_t max_len;
+    float scale;
+} hipdec_attention_rows;
+int hipdec_attention_paged_workspace(uint64_t n_rows, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint64_t max_len,
+                                     uint64_t *out_bytes);
+int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attention_rows *rows, void *d_workspace,
+                           uint64_t workspace_bytes, void *stream);
+
+/* Which of a sequence's drafted tokens the target model keeps, and the token behind them.  Row s * (max_drafts + 1) + i
+ * of d_logits (at that many row_strides) holds the target's logits where draft i of sequence s stands, the row behind
+ * the last draft those of the next token; d_n_drafts[s] (NULL: max_drafts; clamped to 0 .. max_drafts) drafts count.
+ * With p = softmax(softcap(logits) / temperature) and q = the draft's probabilities (d_draft_probs row
+ * s * max_drafts + i; NULL: certain of its token), draft i is kept while d_uniforms[s][i] * q(draft) < p(draft); where
+ * it is not, the next token is drawn from max(p - q, 0) (from p if that is zero everywhere), behind the last kept
+ * draft from p: the lowest index whose running sum exceeds d_uniforms[s][max_drafts] times the whole sum, both in 64
+ * bits.  temperature 0: p is certain of the largest logit (the lowest index of equals) and q of the draft, no random
+ * number is used (d_uniforms may be NULL).  d_tokens[s][max_drafts + 1]: the kept drafts, the next token, then
+ * 0xffffffff; d_accepted[s]: how many drafts were kept.  A draft outside the vocabulary is not kept; NaN logits are
+ * impossible tokens, and so are those of -inf; a row of nothing else gives the next token 0xffffffff.  softcap <= 0:
+ * none.  vocab <= 262144, max_drafts 0 .. 255.  d_workspace: at least hipdec_verify_drafts_workspace bytes, 16-byte
+ * aligned. */
+typedef struct {
+    const void *d_logits;
+    uint32_t dtype, vocab;               /* hipdec_row_dtype */
+    uint64_t n_seqs;
+    uint32_t max_drafts;
+    float temperature, softcap;
+    int64_t row_stride, prob_stride;     /* elements between rows of d_logits / d_draft_probs */
+    const int32_t *d_drafts, *d_n_drafts;
+    const float *d_draft_probs, *d_uniforms;
+    uint32_t *d_tokens;
+    int32_t *d_accepted;
+} hipdec_drafts;
+int hipdec_verify_drafts_workspace(uint64_t n_seqs, uint32_t max_drafts, uint32_t vocab, uint64_t *out_bytes);
+int hipdec_verify_drafts(const hipdec_drafts *drafts, void *d_workspace, uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,4 +1,5 @@
 """Build steps for the native parts: the gfx950 decode library and the host engine above it."""
+import concurrent.futures
 import os
 import subprocess
 
@@ -10,8 +11,9 @@ ENGINE_SO = os.path.join(LIBDIR, "librustane_engine.so")
 GENERATE_BIN = os.path.join(LIBDIR, "generate")
 SERVE_BIN = os.path.join(LIBDIR, "serve")
 
-HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+HIP_SOURCES = ["hip_decode.hip", "serving_ops.hip"]
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fopenmp", "-Wall"]
 
 
@@ -25,7 +27,11 @@ def _run(cmd):
 def build_hipdecode():
     os.makedirs(LIBDIR, exist_ok=True)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    _run([hipcc] + HIP_FLAGS + [os.path.join(CSRC, "hip_decode.hip"), "-o", HIPDECODE_SO])
+    objects = [os.path.join(LIBDIR, os.path.splitext(f)[0] + ".o") for f in HIP_SOURCES]
+    with concurrent.futures.ThreadPoolExecutor(len(HIP_SOURCES)) as pool:
+        list(pool.map(lambda fo: _run([hipcc] + HIP_FLAGS + ["-c", os.path.join(CSRC, fo[0]), "-o", fo[1]]),
+                      zip(HIP_SOURCES, objects)))
+    _run([hipcc, "--offload-arch=gfx950", "-fPIC", "-shared"] + objects + ["-o", HIPDECODE_SO])
     return HIPDECODE_SO
 
 

@@ -38,7 +38,7 @@ struct DevLayer {
     void *kc = nullptr, *vc = nullptr;
 };
 
-std::string g_create_error;
+thread_local std::string g_create_error;   // (per thread: two threads may fail at once)
 
 // Workspace of the chunked prompt prefill (hipdec_prefill.h), allocated at the first prefill.
 struct PrefillWork {
@@ -1384,6 +1384,12 @@ template <typename F> void hostmath_host_range(uint32_t first_bits, uint64_t cou
 }  // namespace
 
 extern "C" {
+
+// errors of the entries without a model that live in other files (serving_ops.hip)
+__attribute__((visibility("hidden"))) int hipdec_op_error(int code, const char *entry, const char *what) {
+    try { g_create_error = std::string(entry) + ": " + what; } catch (...) { g_create_error.clear(); }
+    return code;
+}
 
 const char *hipdec_last_error(const hipdec_model *m) { return m ? m->err.c_str() : g_create_error.c_str(); }
 

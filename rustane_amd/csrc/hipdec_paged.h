@@ -1,0 +1,484 @@
+// A paged key-value cache for gfx950: rotary positions with the append of new rows, and attention of new tokens
+// over the cached ones.  Page p of a pool holds 2^page_shift consecutive slots of one sequence; a sequence's slot s
+// is slot s % page of page page_table[sequence][s / page].
+#pragma once
+#include "hipdec_common.h"
+
+struct PagedView {           // hipdec_paged_cache as the kernels take it: strides in bytes
+    char *k, *v;
+    long long stride_page, stride_slot, stride_head;
+    const int *table;        // [n_seqs][max_pages]
+    int n_pages, page_shift, n_seqs, max_pages, kv_heads;
+};
+
+// page of a sequence's slot; -1 where the table names none of the pool's pages
+__device__ __forceinline__ int pg_page(const PagedView &c, int seq, int slot) {
+    const int p = c.table[(size_t)seq * c.max_pages + (slot >> c.page_shift)];
+    return (unsigned)p < (unsigned)c.n_pages ? p : -1;
+}
+__device__ __forceinline__ long long pg_offset(const PagedView &c, int page, int slot) {
+    return (long long)page * c.stride_page + (long long)(slot & ((1 << c.page_shift) - 1)) * c.stride_slot;
+}
+
+// ---------------------------------------------------------------- rotary positions and the append
+// Row t at position m: pair i of the first `rot` elements of every query and key head turns by the angle m * freq[i]
+// (pair = elements (2i, 2i + 1), or (i, i + rot / 2) in the half layout), both results scaled by `magnitude`; the
+// other elements and the values pass through.  Queries go to q_out, keys and values to the row's slot of the cache.
+// The angle is reduced in 64 bits (m * freq to whole turns: a position of a million in fp32 is off by a tenth of a
+// radian), its sine and cosine and the turn are fp32, and each result is rounded once, to its own type.
+struct RopeArgs {
+    PagedView c;
+    const void *q, *k, *v;
+    void *q_out;
+    long long q_stride, k_stride, v_stride, out_stride;      // elements between rows
+    const double *freq;
+    const int *pos, *slots, *seqs;                           // slots / seqs may be null: the position / the row
+    int heads, kv_heads, hd, rot, interleaved, parts;
+    float magnitude;
+};
+
+template <bool B16> __device__ __forceinline__ float pg_get(const void *p, long long i) {
+    return B16 ? bf16_to_f32(((const uint16_t *)p)[i]) : ((const float *)p)[i];
+}
+template <bool B16, int N> __device__ __forceinline__ void pg_get_n(const void *p, long long i, float *x) {
+    if (N == 1) { x[0] = pg_get<B16>(p, i); return; }
+    if (B16) {
+        const uint2 u = *(const uint2 *)((const uint16_t *)p + i);
+        x[0] = __uint_as_float(u.x << 16); x[1] = __uint_as_float(u.x & 0xffff0000u);
+        x[2] = __uint_as_float(u.y << 16); x[3] = __uint_as_float(u.y & 0xffff0000u);
+    } else {
+        const float4 u = *(const float4 *)((const float *)p + i);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    }
+}
+template <bool B16, int N> __device__ __forceinline__ void pg_put_n(void *p, long long i, const float *x) {
+    if (N == 1) {
+        if (B16) ((uint16_t *)p)[i] = f32_to_bf16_rne(x[0]); else ((float *)p)[i] = x[0];
+        return;
+    }
+    if (B16) {
+        uint2 u;
+        u.x = f32_to_bf16_rne(x[0]) | (uint32_t)f32_to_bf16_rne(x[1]) << 16;
+        u.y = f32_to_bf16_rne(x[2]) | (uint32_t)f32_to_bf16_rne(x[3]) << 16;
+        *(uint2 *)((uint16_t *)p + i) = u;
+    } else {
+        *(float4 *)((float *)p + i) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+}
+
+#define ROPE_THREADS 256
+// One workgroup per row and part of its heads.  A thread keeps one unit (NP pairs) of the head and walks the heads,
+// so that its NP angles are worked out once.  NP = 4 wherever the pieces are 4 aligned elements, else 1.
+template <bool RB, bool CB, int NP> __global__ __launch_bounds__(ROPE_THREADS) void k_rope_append(RopeArgs a) {
+    const int units = a.hd / (2 * NP), per_pass = ROPE_THREADS / units;
+    const int u = threadIdx.x % units, hg = threadIdx.x / units;
+    const int t = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    if (hg >= per_pass) return;
+    const int m = a.pos[t];
+    const int seq = a.seqs ? a.seqs[t] : t, slot = a.slots ? a.slots[t] : m;
+    // a row outside the cache (a padding row: slot < 0; a slot, sequence or page that does not exist) writes nothing
+    long long at = -1;
+    if ((unsigned)seq < (unsigned)a.c.n_seqs && slot >= 0 && (slot >> a.c.page_shift) < a.c.max_pages) {
+        const int page = pg_page(a.c, seq, slot);
+        if (page >= 0) at = pg_offset(a.c, page, slot);
+    }
+    const bool turned = u < a.rot / (2 * NP);
+    float cs[NP], sn[NP];
+    if (turned) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const double turns = (double)m * (a.freq[u * NP + i] * 0.15915494309189533577);
+            sincospif(2.0f * (float)(turns - rint(turns)), &sn[i], &cs[i]);
+            cs[i] *= a.magnitude; sn[i] *= a.magnitude;
+        }
+    }
+    const bool half = turned && !a.interleaved;
+    const int o0 = half ? NP * u : 2 * NP * u, o1 = half ? a.rot / 2 + NP * u : 2 * NP * u + NP;
+    const int H = a.heads, KV = a.kv_heads;
+    for (int h = part * per_pass + hg; h < H + 2 * KV; h += a.parts * per_pass) {
+        const void *src = h < H ? a.q : h < H + KV ? a.k : a.v;
+        const int hh = h < H ? h : h < H + KV ? h - H : h - H - KV;
+        const long long from = (long long)t * (h < H ? a.q_stride : h < H + KV ? a.k_stride : a.v_stride) + (long long)hh * a.hd;
+        if (h >= H && at < 0) continue;
+        const bool turn = turned && h < H + KV;
+        const int p0 = h < H + KV ? o0 : 2 * NP * u, p1 = h < H + KV ? o1 : 2 * NP * u + NP;
+        float x[2 * NP], y[2 * NP];
+        pg_get_n<RB, NP>(src, from + p0, x);
+        pg_get_n<RB, NP>(src, from + p1, x + NP);
+#pragma unroll
+        for (int i = 0; i < 2 * NP; ++i) y[i] = x[i];
+        if (turn) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                if (half) {
+                    y[i] = x[i] * cs[i] - x[NP + i] * sn[i];
+                    y[NP + i] = x[NP + i] * cs[i] + x[i] * sn[i];
+                } else {
+                    y[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
+                    y[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+                }
+            }
+        }
+        if (h < H) {
+            const long long to = (long long)t * a.out_stride + (long long)hh * a.hd;
+            pg_put_n<RB, NP>(a.q_out, to + p0, y);
+            pg_put_n<RB, NP>(a.q_out, to + p1, y + NP);
+        } else {
+            char *base = (h < H + KV ? a.c.k : a.c.v) + at + (long long)hh * a.c.stride_head;
+            pg_put_n<CB, NP>(base, p0, y);
+            pg_put_n<CB, NP>(base, p1, y + NP);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- attention of new tokens over the cache
+// out[row][h] = sum_s w_s v_s, w = softmax over s < len of scale * q[row][h] . k_s, for the g = heads / kv_heads
+// query heads that share a key head at once.  The cache is read once, so the bound is its bytes over HBM's rate.
+//
+// The tile is 16 keys x 16 query heads of the matrix instructions (columns past g idle).  Scores are computed
+// transposed, S^T = K Q^T, so that lane l's result registers are the scores of head l % 16 with keys 4 (l / 16) + r:
+// exactly what the second product, O^T = V^T P^T on the fp32 matrix instruction, wants as its operand, with V read
+// in whole rows as it lies in the cache (lane l holds 16 bytes of key 4 (l / 16) + r, and element e of them is the
+// operand of one instruction).  Probabilities never leave their registers, nothing is transposed, the running
+// maximum and sum of a head sit in the lanes that hold its output, and P and V enter as fp32: a bf16 cache costs no
+// precision beyond its own.  The fp32 instruction has room: 64 cached numbers per 32 clocks and SIMD are 32 bytes a
+// clock and CU of a bf16 cache, three times what HBM delivers.
+//   K of a bf16 cache goes into the bf16 instruction as it is; fp32 queries are three bf16 numbers each (24 bits),
+//   bf16 queries are one.  K of an fp32 cache uses the fp32 instruction.
+struct PagedAttn {
+    PagedView c;
+    const void *q;
+    void *out;
+    long long q_stride, out_stride;                          // elements between rows
+    const int *lens, *seqs;
+    int heads, g, tiles, max_len, chunk, splits;
+    float sc;                                                // scale * log2(e)
+    float *part_o, *part_ml;                                 // splits > 1: [row][head][split][HD], [row][head][split][2]
+};
+
+typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 pg_bf8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ int pg_len(const PagedAttn &a, int row, int &seq) {
+    seq = a.seqs ? a.seqs[row] : row;
+    const int n = a.lens[row];
+    return (unsigned)seq < (unsigned)a.c.n_seqs && n > 0 ? min(n, a.max_len) : 0;
+}
+
+// The keys and values of one block of NT x 16 slots, in registers.
+template <int HD, bool CB, int NT> struct PagedTile {
+    static constexpr int KQ = HD * (CB ? 2 : 4) / 64;        // 16-byte pieces of a key per lane (4 lanes a key)
+    static constexpr int NE = HD / 16;                       // elements of a value per lane (16 lanes a value)
+    static constexpr int VW = CB ? NE / 2 : NE;              // ... in dwords
+    uint4 k[NT][KQ];
+    uint32_t v[NT][4][VW];
+};
+
+#define ATT_WAVES 4
+template <int HD, bool QB, bool CB> __global__ __launch_bounds__(64 * ATT_WAVES) void k_attn_paged(PagedAttn a) {
+    constexpr int NT = HD * (CB ? 2 : 4) <= 256 ? 2 : 1;     // key tiles of a block
+    constexpr int KEYS = 16 * NT;
+    using Tile = PagedTile<HD, CB, NT>;
+    constexpr int KQ = Tile::KQ, NE = Tile::NE, VW = Tile::VW;
+    constexpr int PARTS = QB ? 1 : 3;
+    constexpr int QN = CB ? KQ * PARTS : KQ;
+    __shared__ __align__(16) float sm_o[ATT_WAVES][16][8 * 16 + 4];
+    __shared__ float sm_m[ATT_WAVES][16], sm_l[ATT_WAVES][16];
+
+    const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
+    const int units = a.c.kv_heads * a.tiles, row = rest / units, unit = rest % units;
+    const int kvh = unit / a.tiles, g0 = (unit % a.tiles) * 16, gn = min(16, a.g - g0), head0 = kvh * a.g + g0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+    int seq;
+    const int len = pg_len(a, row, seq);
+    const int lo = split * a.chunk, hi = min(len, lo + a.chunk);
+    if (lo >= hi) {
+        if (a.splits == 1)                                   // nothing to attend to: zeros
+            for (int i = threadIdx.x; i < gn * HD; i += 64 * ATT_WAVES) {
+                const long long at = (long long)row * a.out_stride + (long long)head0 * HD + i;
+                if (QB) ((uint16_t *)a.out)[at] = 0; else ((float *)a.out)[at] = 0.0f;
+            }
+        return;
+    }
+
+    // queries: column `col` of the tile, the reduction elements that this lane's pieces of a key hold
+    uint4 qr[QN];
+    {
+        const long long at = (long long)row * a.q_stride + (long long)(head0 + (col < gn ? col : 0)) * HD;
+#pragma unroll
+        for (int j = 0; j < KQ; ++j) {
+            if (CB) {
+                const long long i = at + 32 * j + 8 * grp;
+                if (QB) {
+                    qr[j] = *(const uint4 *)((const uint16_t *)a.q + i);
+                } else {
+                    const float4 x = *(const float4 *)((const float *)a.q + i), y = *(const float4 *)((const float *)a.q + i + 4);
+                    float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t b0 = f32_to_bf16_rne(f[2 * e]), b1 = f32_to_bf16_rne(f[2 * e + 1]);
+                            w[e] = b0 | b1 << 16;
+                            // (an infinity stays in the first part)
+                            f[2 * e] = (b0 & 0x7f80u) == 0x7f80u ? 0.0f : f[2 * e] - bf16_to_f32(b0);
+                            f[2 * e + 1] = (b1 & 0x7f80u) == 0x7f80u ? 0.0f : f[2 * e + 1] - bf16_to_f32(b1);
+                        }
+                        qr[p * KQ + j] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            } else {
+                const long long i = at + 16 * j + 4 * grp;
+                if (QB) {
+                    const uint2 b = *(const uint2 *)((const uint16_t *)a.q + i);
+                    qr[j] = make_uint4(b.x << 16, b.x & 0xffff0000u, b.y << 16, b.y & 0xffff0000u);
+                } else {
+                    qr[j] = *(const uint4 *)((const float *)a.q + i);
+                }
+            }
+        }
+        if (col >= gn)
+#pragma unroll
+            for (int j = 0; j < QN; ++j) qr[j] = make_uint4(0, 0, 0, 0);
+    }
+
+    const char *kb = a.c.k + (long long)kvh * a.c.stride_head + 16 * grp, *vb = a.c.v + (long long)kvh * a.c.stride_head;
+    // page of the slot that is key `col` of each tile; -1: past the end, or without a page.  What is read for such a
+    // slot lies in page 0 and does not count: its score becomes -inf and its value zero (it may hold a NaN).
+    auto look = [&](int b, int *pg) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int s = lo + b * KEYS + 16 * t + col;
+            pg[t] = s < hi ? pg_page(a.c, seq, s) : -1;
+        }
+    };
+    auto load_k = [&](int b, const int *pg, Tile &x) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int s = lo + b * KEYS + 16 * t + col;
+            const char *p = kb + pg_offset(a.c, max(pg[t], 0), s);
+#pragma unroll
+            for (int j = 0; j < KQ; ++j) x.k[t][j] = *(const uint4 *)(p + 64 * j);
+        }
+    };
+    auto load_v = [&](int b, const int *pg, Tile &x) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int s = lo + b * KEYS + 16 * t + 4 * grp + r;
+                const int page = __shfl(pg[t], 4 * grp + r, WAVE);
+                const char *p = vb + pg_offset(a.c, max(page, 0), s);
+                if (CB) {
+#pragma unroll
+                    for (int c = 0; c < NE / 8; ++c) {
+                        const uint4 w = *(const uint4 *)(p + 256 * c + 16 * col);
+                        x.v[t][r][4 * c] = w.x; x.v[t][r][4 * c + 1] = w.y; x.v[t][r][4 * c + 2] = w.z; x.v[t][r][4 * c + 3] = w.w;
+                    }
+                    if (NE % 8) {
+                        const uint2 w = *(const uint2 *)(p + 256 * (NE / 8) + 8 * col);
+                        x.v[t][r][VW - 2] = w.x; x.v[t][r][VW - 1] = w.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < NE / 4; ++c) {
+                        const uint4 w = *(const uint4 *)(p + 256 * c + 16 * col);
+                        x.v[t][r][4 * c] = w.x; x.v[t][r][4 * c + 1] = w.y; x.v[t][r][4 * c + 2] = w.z; x.v[t][r][4 * c + 3] = w.w;
+                    }
+                }
+            }
+    };
+
+    pg_f4 acc[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) acc[e] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;                           // of head `col`: m the same in its four lanes, l each lane's own share
+    const int blocks = (hi - lo + KEYS - 1) / KEYS;
+    Tile x;
+    int pg[NT], nx[NT];
+    int b = wave;
+    if (b < blocks) {
+        look(b, pg);
+        load_k(b, pg, x);
+        load_v(b, pg, x);
+        look(b + ATT_WAVES, nx);
+    }
+    for (; b < blocks; b += ATT_WAVES) {
+        pg_f4 s[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            s[t] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < KQ; ++j) {
+                if (CB) {
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; --p)
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pg_bf8, x.k[t][j]),
+                                                                       __builtin_bit_cast(pg_bf8, qr[p * KQ + j]), s[t], 0, 0, 0);
+                } else {
+                    const uint32_t kw[4] = {x.k[t][j].x, x.k[t][j].y, x.k[t][j].z, x.k[t][j].w};
+                    const uint32_t qw[4] = {qr[j].x, qr[j].y, qr[j].z, qr[j].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e]), __uint_as_float(qw[e]), s[t], 0, 0, 0);
+                }
+            }
+        }
+        const bool more = b + ATT_WAVES < blocks;
+        bool gaps = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) gaps |= __ballot(pg[t] < 0) != 0;
+        if (more) load_k(b + ATT_WAVES, nx, x);
+        if (gaps)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (__shfl(pg[t], 4 * grp + r, WAVE) < 0) s[t][r] = -INFINITY;
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][r]);
+        top = fmaxf(top, __shfl_xor(top, 16, WAVE));
+        top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+        const float mn = fmaxf(m, top * a.sc);
+        const float ms = mn == -INFINITY ? 0.0f : mn;        // a head without a key so far: every weight is exp2(-inf) = 0
+        const float fall = __builtin_amdgcn_exp2f(m - ms);
+        m = mn;
+        l *= fall;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) acc[e] *= fall;
+        float p[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.sc, -ms));
+                l += p[t][r];
+            }
+        if (gaps)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (__shfl(pg[t], 4 * grp + r, WAVE) < 0)
+#pragma unroll
+                        for (int c = 0; c < VW; ++c) x.v[t][r][c] = 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    const uint32_t w = x.v[t][r][CB ? e / 2 : e];
+                    const float f = __uint_as_float(!CB ? w : e % 2 ? w & 0xffff0000u : w << 16);
+                    acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(f, p[t][r], acc[e], 0, 0, 0);
+                }
+        if (more) {
+            load_v(b + ATT_WAVES, nx, x);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) pg[t] = nx[t];
+            look(b + 2 * ATT_WAVES, nx);
+        }
+    }
+
+    // the waves' shares joined: every wave's output in LDS, 16 dims of a head per element index, summed in wave order
+    l += __shfl_xor(l, 16, WAVE);
+    l += __shfl_xor(l, 32, WAVE);
+    if (grp == 0) { sm_m[wave][col] = m; sm_l[wave][col] = l; }
+    const int head = threadIdx.x >> 4, part = threadIdx.x & 15;
+    float M = -INFINITY, L = 0.0f, wt[ATT_WAVES];
+#pragma unroll
+    for (int e0 = 0; e0 < NE; e0 += CB && NE - e0 >= 8 ? 8 : 4) {
+        const int ce = CB && NE - e0 >= 8 ? 8 : 4;
+        if (e0) __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < ce; e += 4)
+                *(float4 *)&sm_o[wave][col][(4 * grp + r) * ce + e] =
+                    make_float4(acc[e0 + e][r], acc[e0 + e + 1][r], acc[e0 + e + 2][r], acc[e0 + e + 3][r]);
+        __syncthreads();
+        if (e0 == 0) {
+#pragma unroll
+            for (int w = 0; w < ATT_WAVES; ++w) M = fmaxf(M, sm_m[w][head]);
+            const float ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < ATT_WAVES; ++w) { wt[w] = __builtin_amdgcn_exp2f(sm_m[w][head] - ms); L += wt[w] * sm_l[w][head]; }
+        }
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < ce; ++e) o[e] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < ATT_WAVES; ++w)
+#pragma unroll
+            for (int e = 0; e < ce; ++e) o[e] = fmaf(wt[w], sm_o[w][head][part * ce + e], o[e]);
+        if (head < gn) {
+            const int d = 16 * e0 + part * ce;
+            if (a.splits == 1) {
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                const long long at = (long long)row * a.out_stride + (long long)(head0 + head) * HD + d;
+#pragma unroll
+                for (int e = 0; e < ce; e += 4) {
+                    float y[4] = {o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+                    pg_put_n<QB, 4>(a.out, at + e, y);
+                }
+            } else {
+                const size_t slot = ((size_t)row * a.heads + head0 + head) * a.splits + split;
+#pragma unroll
+                for (int e = 0; e < ce; e += 4)
+                    *(float4 *)(a.part_o + slot * HD + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                if (e0 == 0 && part == 0) *(float2 *)(a.part_ml + 2 * slot) = make_float2(M, L);
+            }
+        }
+    }
+}
+
+// The splits of one row and head joined, in the order of the cache within each group of threads.
+template <int HD, bool QB> __global__ __launch_bounds__(256) void k_attn_paged_join(PagedAttn a) {
+    constexpr int W = HD / 4, G = 256 / W;                   // threads across a head, groups that take every G-th split
+    __shared__ __align__(16) float sm[G][HD];
+    __shared__ float sm_l[G], sm_top[4];
+    const int row = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+    int seq;
+    const int len = pg_len(a, row, seq);
+    const int n = (len + a.chunk - 1) / a.chunk;
+    const size_t slot0 = ((size_t)row * a.heads + h) * a.splits;
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, a.part_ml[2 * (slot0 + i)]);
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) sm_top[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sm_top[0], sm_top[1]), fmaxf(sm_top[2], sm_top[3]));
+    if (top == -INFINITY) top = 0.0f;
+    const int grp = threadIdx.x / W, d = (threadIdx.x % W) * 4;
+    if (grp < G) {
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+        for (int i = grp; i < n; i += G) {
+            const float2 ml = *(const float2 *)(a.part_ml + 2 * (slot0 + i));
+            const float4 x = *(const float4 *)(a.part_o + (slot0 + i) * HD + d);
+            const float w = __builtin_amdgcn_exp2f(ml.x - top);
+            l = fmaf(w, ml.y, l);
+            o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+        }
+        *(float4 *)&sm[grp][d] = o;
+        if (d == 0) sm_l[grp] = l;
+    }
+    __syncthreads();
+    if (grp == 0) {
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+            l += sm_l[k];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] += sm[k][d + e];
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= inv;
+        pg_put_n<QB, 4>(a.out, (long long)row * a.out_stride + (long long)h * HD + d, y);
+    }
+}

@@ -1,0 +1,268 @@
+// The C entries of the operators on the caller's device buffers (include/hip_decode.h): argument checks, the choice
+// of kernel and launch.  Nothing here allocates, waits or keeps state between calls.
+#include "../../include/hip_decode.h"
+#include "hipdec_paged.h"
+#include "hipdec_verify.h"
+
+#include <math.h>
+#include <stdio.h>
+
+// hip_decode.hip: sets the text hipdec_last_error(NULL) returns on this thread
+extern "C" __attribute__((visibility("hidden"))) int hipdec_op_error(int code, const char *entry, const char *what);
+
+namespace {
+
+constexpr uint32_t kMaxPage = 65536, kMaxHeadDim = 512, kMaxVocab = 262144, kMaxDrafts = 255;
+constexpr uint64_t kMaxRows = 1u << 24, kMaxLen = 1u << 30;
+constexpr int kCus = 256;                                    // compute units of the one device this is built for
+
+int refuse(const char *entry, const char *what) { return hipdec_op_error(HIPDEC_ERR_ARG, entry, what); }
+int launched(const char *entry) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? HIPDEC_OK : hipdec_op_error(HIPDEC_ERR_HIP, entry, hipGetErrorString(e));
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// Whether `p` is memory that kernels of the current device may use, and `stream` one of its streams: a host pointer,
+// or a buffer of another device, would end the process inside a kernel.
+const char *wrong_place(std::initializer_list<const void *> buffers, void *stream) {
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess) { (void)hipGetLastError(); return "no current device"; }
+    if (stream) {
+        hipDevice_t of = -1;
+        if (hipStreamGetDevice((hipStream_t)stream, &of) != hipSuccess) { (void)hipGetLastError(); return "not a stream"; }
+        if ((int)of != dev) return "the stream is of another device than the current one";
+    }
+    for (const void *p : buffers) {
+        if (!p) continue;
+        hipPointerAttribute_t at{};
+        if (hipPointerGetAttributes(&at, p) != hipSuccess) { (void)hipGetLastError(); return "a buffer is not device memory"; }
+        if (at.type == hipMemoryTypeDevice ? at.device != dev : at.type != hipMemoryTypeManaged && at.type != hipMemoryTypeHost)
+            return at.type == hipMemoryTypeDevice ? "a buffer is of another device than the current one" : "a buffer is not device memory";
+    }
+    return nullptr;
+}
+
+const char *check_cache(const hipdec_paged_cache *c) {
+    if (!c->k || !c->v || !c->page_table) return "null buffer in the cache";
+    if (c->kv_dtype > HIPDEC_KV_BF16) return "unknown kv_dtype";
+    if (!c->n_pages || !c->kv_heads || !c->hd || !c->n_seqs || !c->max_pages) return "zero-sized cache";
+    if (c->n_pages > 0x7fffffffu || c->n_seqs > kMaxRows || c->max_pages > 0x7fffffffu || c->kv_heads > 65536) return "cache too large";
+    if (!c->page_size || (c->page_size & (c->page_size - 1)) || c->page_size > kMaxPage) return "page_size must be a power of two up to 65536";
+    if (c->stride_page < 0 || c->stride_slot < 0 || c->stride_head < 0) return "negative stride";
+    return nullptr;
+}
+
+PagedView view(const hipdec_paged_cache &c) {
+    const long long e = c.kv_dtype == HIPDEC_KV_BF16 ? 2 : 4;
+    PagedView v{(char *)c.k, (char *)c.v, c.stride_page * e, c.stride_slot * e, c.stride_head * e, c.page_table,
+                (int)c.n_pages, 0, (int)c.n_seqs, (int)c.max_pages, (int)c.kv_heads};
+    while ((1u << v.page_shift) < c.page_size) ++v.page_shift;
+    return v;
+}
+
+// Keys per split of the cache's length: a multiple of what the workgroup's waves take at once.
+struct Split { int chunk, splits; };
+Split split_of(uint64_t n_rows, uint32_t kv_heads, uint32_t g, uint64_t max_len) {
+    const uint64_t units = n_rows * kv_heads * ((g + 15) / 16), steps = (max_len + 127) / 128;
+    uint64_t per = (units * steps + 4 * kCus - 1) / (4 * kCus);
+    if (per < 1) per = 1;
+    if (per > 8) per = 8;
+    if (steps <= per) return Split{(int)(steps ? steps : 1) * 128, 1};
+    return Split{(int)per * 128, (int)((steps + per - 1) / per)};
+}
+
+template <int HD, bool QB, bool CB> void go_attention(const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
+    hipLaunchKernelGGL((k_attn_paged<HD, QB, CB>), dim3(grid), dim3(64 * ATT_WAVES), 0, s, a);
+    if (joins) hipLaunchKernelGGL((k_attn_paged_join<HD, QB>), dim3(joins), dim3(256), 0, s, a);
+}
+template <int HD> void go_attention(bool qb, bool cb, const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
+    if (qb) { if (cb) go_attention<HD, true, true>(a, grid, joins, s); else go_attention<HD, true, false>(a, grid, joins, s); }
+    else { if (cb) go_attention<HD, false, true>(a, grid, joins, s); else go_attention<HD, false, false>(a, grid, joins, s); }
+}
+
+template <bool RB, bool CB> void go_rope(const RopeArgs &a, bool wide, unsigned grid, hipStream_t s) {
+    if (wide) hipLaunchKernelGGL((k_rope_append<RB, CB, 4>), dim3(grid), dim3(ROPE_THREADS), 0, s, a);
+    else hipLaunchKernelGGL((k_rope_append<RB, CB, 1>), dim3(grid), dim3(ROPE_THREADS), 0, s, a);
+}
+
+uint64_t chunks_of(uint32_t vocab) { return (vocab + VF_CHUNK - 1) / VF_CHUNK; }
+
+template <bool B16> void go_verify(const VerifyArgs &a, bool rest, hipStream_t s) {
+    const unsigned rows = (unsigned)a.n_seqs * (a.max_drafts + 1);
+    hipLaunchKernelGGL(k_verify_stats<B16>, dim3(rows * a.chunks), dim3(VF_THREADS), 0, s, a);
+    if (rest) hipLaunchKernelGGL(k_verify_sums<B16>, dim3((unsigned)a.n_seqs * a.chunks), dim3(VF_THREADS), 0, s, a);
+    hipLaunchKernelGGL(k_verify_draw<B16>, dim3((unsigned)a.n_seqs), dim3(VF_THREADS), 0, s, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int hipdec_rope_frequencies(uint32_t scaling, uint32_t rot_dim, double theta, double factor, double trained,
+                            double slow_turns, double fast_turns, double *freq, float *magnitude) {
+    const char *me = "hipdec_rope_frequencies";
+    if (!freq || !magnitude) return refuse(me, "null buffer");
+    if (scaling > HIPDEC_ROPE_PARTS) return refuse(me, "unknown scaling");
+    if (rot_dim == 0 || rot_dim % 2 || rot_dim > kMaxHeadDim) return refuse(me, "rot_dim must be even, 2 .. 512");
+    if (!(theta > 1.0) || !isfinite(theta)) return refuse(me, "theta must be above 1");
+    if (scaling != HIPDEC_ROPE_PLAIN && (!(factor >= 1.0) || !isfinite(factor))) return refuse(me, "factor must be at least 1");
+    if (scaling == HIPDEC_ROPE_BASE && rot_dim == 2) return refuse(me, "one pair cannot be scaled by its base");
+    if (scaling == HIPDEC_ROPE_PARTS && (!(trained > 0.0) || !isfinite(trained) || !(slow_turns >= 0.0) || !(fast_turns > slow_turns) || !isfinite(fast_turns)))
+        return refuse(me, "trained must be above 0 and fast_turns above slow_turns, which is not negative");
+    if (scaling == HIPDEC_ROPE_BASE) theta *= pow(factor, (double)rot_dim / (rot_dim - 2));
+    for (uint32_t i = 0; i < rot_dim / 2; ++i) {
+        double f = pow(theta, -2.0 * i / rot_dim);
+        if (scaling == HIPDEC_ROPE_LINEAR) f /= factor;
+        if (scaling == HIPDEC_ROPE_PARTS) {
+            const double turns = trained * f / 6.283185307179586477;
+            const double keep = fmin(fmax((turns - slow_turns) / (fast_turns - slow_turns), 0.0), 1.0);
+            f = f * keep + f / factor * (1.0 - keep);
+        }
+        freq[i] = f;
+    }
+    *magnitude = scaling == HIPDEC_ROPE_PARTS ? (float)(0.1 * log(factor) + 1.0) : 1.0f;
+    return HIPDEC_OK;
+}
+
+int hipdec_rope_append_paged(const hipdec_rope *rope, const hipdec_paged_cache *cache, const hipdec_new_rows *rows,
+                             void *stream) {
+    const char *me = "hipdec_rope_append_paged", *bad;
+    if (!rope || !cache || !rows) return refuse(me, "null argument");
+    if ((bad = check_cache(cache))) return refuse(me, bad);
+    if (rows->n_rows == 0) return HIPDEC_OK;
+    if (!rows->d_q || !rows->d_k || !rows->d_v || !rows->d_q_out || !rows->d_positions || (rope->rot_dim && !rope->d_freq))
+        return refuse(me, "null buffer");
+    if (rows->dtype > HIPDEC_ROWS_BF16) return refuse(me, "unknown dtype");
+    if (!rows->heads || rows->heads > 65536 || rows->n_rows > kMaxRows) return refuse(me, "heads or n_rows out of range");
+    if (cache->hd % 2 || cache->hd > kMaxHeadDim) return refuse(me, "hd must be even, up to 512");
+    if (rope->rot_dim % 2 || rope->rot_dim > cache->hd) return refuse(me, "rot_dim must be even, up to hd");
+    if (!isfinite(rope->magnitude)) return refuse(me, "magnitude must be finite");
+    const int64_t wide_q = (int64_t)rows->heads * cache->hd, wide_k = (int64_t)cache->kv_heads * cache->hd;
+    if (rows->n_rows > 1 && (rows->q_stride < wide_q || rows->q_out_stride < wide_q || rows->k_stride < wide_k || rows->v_stride < wide_k))
+        return refuse(me, "rows overlap: a stride is smaller than its row");
+    if (rows->d_q == rows->d_q_out && rows->q_stride != rows->q_out_stride) return refuse(me, "in place, both strides must be equal");
+    if ((bad = wrong_place({rows->d_q, rows->d_k, rows->d_v, rows->d_q_out, rows->d_positions, rows->d_slots, rows->d_seqs, rope->d_freq,
+                            cache->k, cache->v, cache->page_table}, stream)))
+        return refuse(me, bad);
+
+    RopeArgs a{view(*cache), rows->d_q, rows->d_k, rows->d_v, rows->d_q_out, rows->q_stride, rows->k_stride, rows->v_stride,
+               rows->q_out_stride, rope->d_freq, rows->d_positions, rows->d_slots, rows->d_seqs, (int)rows->heads,
+               (int)cache->kv_heads, (int)cache->hd, (int)rope->rot_dim, rope->interleaved != 0, 1, rope->magnitude};
+    const int64_t strides = rows->q_stride | rows->k_stride | rows->v_stride | rows->q_out_stride | cache->stride_page |
+                            cache->stride_slot | cache->stride_head;
+    const bool wide = cache->hd % 8 == 0 && rope->rot_dim % 8 == 0 && strides % 4 == 0 && aligned16(rows->d_q) && aligned16(rows->d_k) &&
+                      aligned16(rows->d_v) && aligned16(rows->d_q_out) && aligned16(cache->k) && aligned16(cache->v);
+    // few rows: a workgroup for every pass over the heads, so that one token's heads run side by side
+    const int per_pass = ROPE_THREADS / (int)(cache->hd / (wide ? 8 : 2));
+    const int passes = (a.heads + 2 * a.kv_heads + per_pass - 1) / per_pass;
+    a.parts = rows->n_rows * passes <= 4 * kCus ? passes : 1;
+    const uint64_t grid = rows->n_rows * a.parts;
+    const bool rb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;
+    hipStream_t s = (hipStream_t)stream;
+    if (rb) { if (cb) go_rope<true, true>(a, wide, (unsigned)grid, s); else go_rope<true, false>(a, wide, (unsigned)grid, s); }
+    else { if (cb) go_rope<false, true>(a, wide, (unsigned)grid, s); else go_rope<false, false>(a, wide, (unsigned)grid, s); }
+    return launched(me);
+}
+
+int hipdec_attention_paged_workspace(uint64_t n_rows, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint64_t max_len,
+                                     uint64_t *out_bytes) {
+    const char *me = "hipdec_attention_paged_workspace";
+    if (!out_bytes) return refuse(me, "null argument");
+    if (!heads || !kv_heads || heads % kv_heads || heads > 65536 || hd > kMaxHeadDim || n_rows > kMaxRows || max_len > kMaxLen)
+        return refuse(me, "heads, hd, n_rows or max_len out of range");
+    const Split p = split_of(n_rows, kv_heads, heads / kv_heads, max_len);
+    *out_bytes = p.splits == 1 ? 0 : n_rows * heads * p.splits * (hd + 2) * sizeof(float);
+    return HIPDEC_OK;
+}
+
+int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attention_rows *rows, void *d_workspace,
+                           uint64_t workspace_bytes, void *stream) {
+    const char *me = "hipdec_attention_paged", *bad;
+    if (!cache || !rows) return refuse(me, "null argument");
+    if ((bad = check_cache(cache))) return refuse(me, bad);
+    if (rows->n_rows == 0) return HIPDEC_OK;
+    if (!rows->d_q || !rows->d_out || !rows->d_lens) return refuse(me, "null buffer");
+    if (rows->dtype > HIPDEC_ROWS_BF16) return refuse(me, "unknown dtype");
+    if (!rows->heads || rows->heads % cache->kv_heads || rows->heads > 65536) return refuse(me, "heads must be a multiple of the cache's kv_heads");
+    if (rows->n_rows > kMaxRows || rows->max_len > kMaxLen) return refuse(me, "n_rows or max_len out of range");
+    if (!(rows->scale > 0.0f) || !isfinite(rows->scale)) return refuse(me, "scale must be above 0");
+    if (cache->hd != 64 && cache->hd != 128 && cache->hd != 192 && cache->hd != 256)
+        return hipdec_op_error(HIPDEC_ERR_UNSUPPORTED, me, "head dim must be 64, 128, 192 or 256");
+    const int64_t wide = (int64_t)rows->heads * cache->hd;
+    if (rows->n_rows > 1 && (rows->q_stride < wide || rows->out_stride < wide)) return refuse(me, "rows overlap: a stride is smaller than its row");
+    const int64_t row_unit = rows->dtype == HIPDEC_ROWS_BF16 ? 8 : 4, kv_unit = cache->kv_dtype == HIPDEC_KV_BF16 ? 8 : 4;
+    if (!aligned16(rows->d_q) || !aligned16(rows->d_out) || !aligned16(cache->k) || !aligned16(cache->v) ||
+        (rows->q_stride | rows->out_stride) % row_unit || (cache->stride_page | cache->stride_slot | cache->stride_head) % kv_unit)
+        return refuse(me, "queries, outputs and the cache must be 16-byte aligned, with strides of whole 16 bytes");
+
+    const uint64_t slots = (uint64_t)cache->max_pages * cache->page_size;
+    const Split p = split_of(rows->n_rows, cache->kv_heads, rows->heads / cache->kv_heads, rows->max_len);
+    const uint64_t need = p.splits == 1 ? 0 : rows->n_rows * rows->heads * p.splits * (cache->hd + 2) * sizeof(float);
+    if (need && (!d_workspace || workspace_bytes < need || !aligned16(d_workspace)))
+        return refuse(me, "workspace missing, too small (hipdec_attention_paged_workspace) or not 16-byte aligned");
+    if ((bad = wrong_place({rows->d_q, rows->d_out, rows->d_lens, rows->d_seqs, cache->k, cache->v, cache->page_table,
+                            need ? d_workspace : nullptr}, stream)))
+        return refuse(me, bad);
+
+    const int g = (int)(rows->heads / cache->kv_heads), tiles = (g + 15) / 16;
+    const uint64_t grid = rows->n_rows * cache->kv_heads * tiles * p.splits, joins = rows->n_rows * rows->heads;
+    if (grid > 0x7fffffffu || joins > 0x7fffffffu) return refuse(me, "n_rows * heads * max_len out of range");
+    float *po = (float *)d_workspace;
+    PagedAttn a{view(*cache), rows->d_q, rows->d_out, rows->q_stride, rows->out_stride, rows->d_lens, rows->d_seqs, (int)rows->heads,
+                g, tiles, (int)(rows->max_len < slots ? rows->max_len : slots), p.chunk, p.splits,
+                rows->scale * 1.44269504088896340736f, po, po + rows->n_rows * rows->heads * p.splits * cache->hd};
+    const bool qb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;
+    const unsigned nj = p.splits > 1 ? (unsigned)joins : 0;
+    hipStream_t s = (hipStream_t)stream;
+    switch (cache->hd) {
+    case 64: go_attention<64>(qb, cb, a, (unsigned)grid, nj, s); break;
+    case 128: go_attention<128>(qb, cb, a, (unsigned)grid, nj, s); break;
+    case 192: go_attention<192>(qb, cb, a, (unsigned)grid, nj, s); break;
+    default: go_attention<256>(qb, cb, a, (unsigned)grid, nj, s); break;
+    }
+    return launched(me);
+}
+
+int hipdec_verify_drafts_workspace(uint64_t n_seqs, uint32_t max_drafts, uint32_t vocab, uint64_t *out_bytes) {
+    const char *me = "hipdec_verify_drafts_workspace";
+    if (!out_bytes) return refuse(me, "null argument");
+    if (max_drafts > kMaxDrafts || n_seqs > kMaxRows || !vocab || vocab > kMaxVocab) return refuse(me, "n_seqs, max_drafts or vocab out of range");
+    *out_bytes = n_seqs * chunks_of(vocab) * ((max_drafts + 1) * sizeof(VfStat) + sizeof(double));
+    return HIPDEC_OK;
+}
+
+int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t workspace_bytes, void *stream) {
+    const char *me = "hipdec_verify_drafts", *bad;
+    if (!d) return refuse(me, "null argument");
+    if (d->n_seqs == 0) return HIPDEC_OK;
+    const bool greedy = d->temperature == 0.0f;
+    if (!d->d_logits || !d->d_tokens || !d->d_accepted || (d->max_drafts && !d->d_drafts) || (!greedy && !d->d_uniforms))
+        return refuse(me, "null buffer");
+    if (d->dtype > HIPDEC_ROWS_BF16) return refuse(me, "unknown dtype");
+    if (!(d->temperature >= 0.0f) || !isfinite(d->temperature)) return refuse(me, "temperature must not be negative");
+    if (!(d->softcap <= 3.4e38f)) return refuse(me, "softcap must be finite");
+    if (d->max_drafts > kMaxDrafts || d->n_seqs > kMaxRows || !d->vocab || d->vocab > kMaxVocab)
+        return refuse(me, "n_seqs, max_drafts or vocab out of range");
+    if (d->row_stride < d->vocab || (d->d_draft_probs && d->max_drafts && d->prob_stride < d->vocab))
+        return refuse(me, "rows overlap: a stride is smaller than the vocabulary");
+    const uint64_t chunks = chunks_of(d->vocab), rows = d->n_seqs * (d->max_drafts + 1);
+    const uint64_t need = d->n_seqs * chunks * ((d->max_drafts + 1) * sizeof(VfStat) + sizeof(double));
+    if (!d_workspace || workspace_bytes < need || !aligned16(d_workspace))
+        return refuse(me, "workspace missing, too small (hipdec_verify_drafts_workspace) or not 16-byte aligned");
+    if (rows * chunks > 0x7fffffffu) return refuse(me, "n_seqs * max_drafts * vocab out of range");
+    if ((bad = wrong_place({d->d_logits, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms, d->d_tokens, d->d_accepted,
+                            d_workspace}, stream)))
+        return refuse(me, bad);
+    VfStat *st = (VfStat *)d_workspace;
+    const VerifyArgs a{d->d_logits, d->row_stride, d->prob_stride, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms,
+                       (int)d->n_seqs, (int)d->max_drafts, (int)d->vocab, (int)chunks, greedy ? 0.0 : 1.0 / (double)d->temperature,
+                       d->softcap, st, (double *)(st + rows * chunks), d->d_tokens, d->d_accepted};
+    const bool rest = !greedy && d->max_drafts;
+    if (d->dtype == HIPDEC_ROWS_BF16) go_verify<true>(a, rest, (hipStream_t)stream);
+    else go_verify<false>(a, rest, (hipStream_t)stream);
+    return launched(me);
+}
+
+}  // extern "C"

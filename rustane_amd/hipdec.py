@@ -35,6 +35,8 @@ EXPORTS = [
     "hipdec_debug_hostmath_count_mismatch", "hipdec_debug_hostmath_probe", "hipdec_debug_sample_topk",
     "hipdec_debug_sample_fullvocab", "hipdec_sample_fullvocab_noalloc", "hipdec_debug_set_spin_limit", "hipdec_debug_step_kernel",
     "hipdec_debug_gemm_plan",
+    "hipdec_rope_frequencies", "hipdec_rope_append_paged", "hipdec_attention_paged_workspace", "hipdec_attention_paged",
+    "hipdec_verify_drafts_workspace", "hipdec_verify_drafts",
 ]
 
 
@@ -48,6 +50,21 @@ class WeightDtype(enum.IntEnum):
 class KvDtype(enum.IntEnum):
     F32 = 0
     BF16 = 1
+
+
+class RowDtype(enum.IntEnum):
+    F32 = 0
+    BF16 = 1
+
+
+class RopeScaling(enum.IntEnum):
+    PLAIN = 0
+    LINEAR = 1
+    BASE = 2
+    PARTS = 3
+
+
+NO_TOKEN = 0xFFFFFFFF        # behind the last token of a verified draft; the next token of a row without a possible one
 
 
 class HipDecodeError(RuntimeError):
@@ -128,6 +145,13 @@ def load_library(path=None):
     lib.hipdec_debug_step_profile.argtypes = [C.c_void_p, C.c_uint32, C.POINTER(C.c_uint64), C.c_size_t,
                                               C.POINTER(C.c_size_t)]
     lib.hipdec_debug_calibration_copy.argtypes = [C.c_size_t, C.c_int]
+    u64p, dbl = C.POINTER(C.c_uint64), C.c_double
+    lib.hipdec_rope_frequencies.argtypes = [C.c_uint32, C.c_uint32, dbl, dbl, dbl, dbl, dbl, C.POINTER(dbl), fp]
+    lib.hipdec_rope_append_paged.argtypes = [C.POINTER(Rope), C.POINTER(PagedCache), C.POINTER(_NewRows), C.c_void_p]
+    lib.hipdec_attention_paged_workspace.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64, u64p]
+    lib.hipdec_attention_paged.argtypes = [C.POINTER(PagedCache), C.POINTER(_AttentionRows), C.c_void_p, C.c_uint64, C.c_void_p]
+    lib.hipdec_verify_drafts_workspace.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32, u64p]
+    lib.hipdec_verify_drafts.argtypes = [C.POINTER(_Drafts), C.c_void_p, C.c_uint64, C.c_void_p]
     szp = C.POINTER(C.c_size_t)
     lib.hipdec_batch_begin.argtypes = [C.c_void_p, C.c_size_t]
     lib.hipdec_batch_end.argtypes = [C.c_void_p]
@@ -223,6 +247,114 @@ def sample_fullvocab_noalloc(d_logits, vocab, d_maxes, d_sums, temperature, d_rn
                                                         d_rng_state, d_out_token, stream)
     if rc != OK:
         raise HipDecodeError(rc, (load_library().hipdec_last_error(None) or b"").decode())
+
+
+# ---- operators on the caller's device buffers.  Every pointer is a device address (an int), `stream` a hipStream_t as
+# an int (None: the default stream); calls enqueue and return without waiting.
+class PagedCache(C.Structure):
+    """hipdec_paged_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("kv_dtype", C.c_uint32), ("page_size", C.c_uint32),
+                ("n_pages", C.c_uint32), ("kv_heads", C.c_uint32), ("hd", C.c_uint32), ("n_seqs", C.c_uint32),
+                ("max_pages", C.c_uint32), ("page_table", C.c_void_p), ("stride_page", C.c_int64),
+                ("stride_slot", C.c_int64), ("stride_head", C.c_int64)]
+
+    @classmethod
+    def make(cls, k, v, kv_dtype, n_pages, page_size, kv_heads, hd, page_table, n_seqs, max_pages, token_major=False,
+             strides=None):
+        """Pools of [page][kv head][slot][hd], with token_major of [page][slot][kv head][hd]; `strides` (page, slot,
+        head, in elements) for any other."""
+        page, slot, head = strides or ((page_size * kv_heads * hd,) +
+                                       ((kv_heads * hd, hd) if token_major else (hd, page_size * hd)))
+        return cls(k, v, kv_dtype, page_size, n_pages, kv_heads, hd, n_seqs, max_pages, page_table, page, slot, head)
+
+
+class Rope(C.Structure):
+    """hipdec_rope."""
+    _fields_ = [("d_freq", C.c_void_p), ("rot_dim", C.c_uint32), ("interleaved", C.c_uint32), ("magnitude", C.c_float)]
+
+    @classmethod
+    def make(cls, d_freq, rot_dim, interleaved=True, magnitude=1.0):
+        return cls(d_freq, rot_dim, 1 if interleaved else 0, magnitude)
+
+
+class _NewRows(C.Structure):
+    _fields_ = [("d_q", C.c_void_p), ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("d_q_out", C.c_void_p),
+                ("dtype", C.c_uint32), ("heads", C.c_uint32), ("n_rows", C.c_uint64), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64),
+                ("d_positions", C.c_void_p), ("d_slots", C.c_void_p), ("d_seqs", C.c_void_p)]
+
+
+class _AttentionRows(C.Structure):
+    _fields_ = [("d_q", C.c_void_p), ("d_out", C.c_void_p), ("dtype", C.c_uint32), ("heads", C.c_uint32),
+                ("n_rows", C.c_uint64), ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("d_lens", C.c_void_p),
+                ("d_seqs", C.c_void_p), ("max_len", C.c_uint64), ("scale", C.c_float)]
+
+
+class _Drafts(C.Structure):
+    _fields_ = [("d_logits", C.c_void_p), ("dtype", C.c_uint32), ("vocab", C.c_uint32), ("n_seqs", C.c_uint64),
+                ("max_drafts", C.c_uint32), ("temperature", C.c_float), ("softcap", C.c_float),
+                ("row_stride", C.c_int64), ("prob_stride", C.c_int64), ("d_drafts", C.c_void_p),
+                ("d_n_drafts", C.c_void_p), ("d_draft_probs", C.c_void_p), ("d_uniforms", C.c_void_p),
+                ("d_tokens", C.c_void_p), ("d_accepted", C.c_void_p)]
+
+
+def _op_chk(lib, rc):
+    if rc != OK:
+        raise HipDecodeError(rc, (lib.hipdec_last_error(None) or b"").decode())
+
+
+def rope_frequencies(rot_dim, theta=10000.0, scaling=RopeScaling.PLAIN, factor=1.0, trained=4096.0, slow_turns=1.0,
+                     fast_turns=32.0):
+    """(angles per position as a float64 array of rot_dim / 2, magnitude); no GPU needed."""
+    lib = load_library()
+    freq, mag = np.empty(max(int(rot_dim) // 2, 1), np.float64), C.c_float()
+    _op_chk(lib, lib.hipdec_rope_frequencies(scaling, rot_dim, theta, factor, trained, slow_turns, fast_turns,
+                                             freq.ctypes.data_as(C.POINTER(C.c_double)), C.byref(mag)))
+    return freq, mag.value
+
+
+def rope_append_paged(rope, cache, q, k, v, q_out, positions, n_rows, heads, dtype=RowDtype.F32, slots=None, seqs=None,
+                      row_stride=None, q_stride=None, k_stride=None, v_stride=None, q_out_stride=None, stream=None):
+    """hipdec_rope_append_paged.  Strides in elements; row_stride stands for those of q, k and v where the three lie in
+    one row (a fused projection); left out, rows are dense."""
+    lib = load_library()
+    wide, kv_wide = heads * cache.hd, cache.kv_heads * cache.hd
+    rows = _NewRows(q, k, v, q_out, dtype, heads, n_rows, q_stride or row_stride or wide, k_stride or row_stride or kv_wide,
+                    v_stride or row_stride or kv_wide, q_out_stride or wide, positions, slots, seqs)
+    _op_chk(lib, lib.hipdec_rope_append_paged(C.byref(rope), C.byref(cache), C.byref(rows), stream))
+
+
+def attention_paged_workspace(n_rows, heads, kv_heads, hd, max_len):
+    """Bytes of device workspace hipdec_attention_paged needs for these sizes; no GPU needed."""
+    lib, out = load_library(), C.c_uint64()
+    _op_chk(lib, lib.hipdec_attention_paged_workspace(n_rows, heads, kv_heads, hd, max_len, C.byref(out)))
+    return out.value
+
+
+def attention_paged(cache, q, out, lens, n_rows, heads, max_len, dtype=RowDtype.F32, scale=None, seqs=None, q_stride=None,
+                    out_stride=None, workspace=None, workspace_bytes=0, stream=None):
+    """hipdec_attention_paged; scale: 1 / sqrt(hd) if left out, strides in elements (dense rows if left out)."""
+    lib = load_library()
+    rows = _AttentionRows(q, out, dtype, heads, n_rows, q_stride or heads * cache.hd, out_stride or heads * cache.hd, lens,
+                          seqs, max_len, cache.hd ** -0.5 if scale is None else scale)
+    _op_chk(lib, lib.hipdec_attention_paged(C.byref(cache), C.byref(rows), workspace, workspace_bytes, stream))
+
+
+def verify_drafts_workspace(n_seqs, max_drafts, vocab):
+    """Bytes of device workspace hipdec_verify_drafts needs for these sizes; no GPU needed."""
+    lib, out = load_library(), C.c_uint64()
+    _op_chk(lib, lib.hipdec_verify_drafts_workspace(n_seqs, max_drafts, vocab, C.byref(out)))
+    return out.value
+
+
+def verify_drafts(logits, drafts, uniforms, tokens, accepted, n_seqs, max_drafts, vocab, dtype=RowDtype.F32, temperature=1.0,
+                  softcap=0.0, n_drafts=None, draft_probs=None, row_stride=None, prob_stride=None, workspace=None,
+                  workspace_bytes=0, stream=None):
+    """hipdec_verify_drafts; strides in elements (dense rows if left out)."""
+    lib = load_library()
+    d = _Drafts(logits, dtype, vocab, n_seqs, max_drafts, temperature, softcap, row_stride or vocab, prob_stride or vocab,
+                drafts, n_drafts, draft_probs, uniforms, tokens, accepted)
+    _op_chk(lib, lib.hipdec_verify_drafts(C.byref(d), workspace, workspace_bytes, stream))
 
 
 def calibration_copy(nbytes, reps=1):
