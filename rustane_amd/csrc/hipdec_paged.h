@@ -159,10 +159,13 @@ struct PagedAttn {
 typedef float pg_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 pg_bf8 __attribute__((ext_vector_type(8)));
 
+// slots that row attends to; seq: its sequence (0 where there is none of that number: no slots then)
 __device__ __forceinline__ int pg_len(const PagedAttn &a, int row, int &seq) {
     seq = a.seqs ? a.seqs[row] : row;
     const int n = a.lens[row];
-    return (unsigned)seq < (unsigned)a.c.n_seqs && n > 0 ? min(n, a.max_len) : 0;
+    if ((unsigned)seq < (unsigned)a.c.n_seqs) return min(max(n, 0), a.max_len);
+    seq = 0;
+    return 0;
 }
 
 // The keys and values of one block of NT x 16 slots, in registers.
@@ -175,23 +178,38 @@ template <int HD, bool CB, int NT> struct PagedTile {
 };
 
 #define ATT_WAVES 4
-template <int HD, bool QB, bool CB> __global__ __launch_bounds__(64 * ATT_WAVES) void k_attn_paged(PagedAttn a) {
-    constexpr int NT = HD * (CB ? 2 : 4) <= 256 ? 2 : 1;     // key tiles of a block
+constexpr int att_tiles(int hd, bool cb) { return hd * (cb ? 2 : 4) <= 128 ? 2 : 1; }
+constexpr int att_groups(int hd, bool cb) { return hd * (cb ? 2 : 4) <= 256 ? 3 : hd * (cb ? 2 : 4) <= 512 ? 2 : 1; }
+template <int HD, bool QB, bool CB, bool FEW> __global__ __launch_bounds__(64 * ATT_WAVES, att_groups(HD, CB)) void k_attn_paged(PagedAttn a) {
+    constexpr int NT = att_tiles(HD, CB);                    // key tiles of a block
     constexpr int KEYS = 16 * NT;
     using Tile = PagedTile<HD, CB, NT>;
     constexpr int KQ = Tile::KQ, NE = Tile::NE, VW = Tile::VW;
     constexpr int PARTS = QB ? 1 : 3;
     constexpr int QN = CB ? KQ * PARTS : KQ;
-    __shared__ __align__(16) float sm_o[ATT_WAVES][16][8 * 16 + 4];
+    __shared__ __align__(16) float sm_o[ATT_WAVES * 16][8 * 16 + 4];
     __shared__ float sm_m[ATT_WAVES][16], sm_l[ATT_WAVES][16];
 
-    const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
+    const unsigned per = gridDim.x / a.splits;               // rows x units
+    const int split = blockIdx.x / per, rest = blockIdx.x % per;
     const int units = a.c.kv_heads * a.tiles, row = rest / units, unit = rest % units;
     const int kvh = unit / a.tiles, g0 = (unit % a.tiles) * 16, gn = min(16, a.g - g0), head0 = kvh * a.g + g0;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+    const int qcol = FEW ? col & 3 : col;                    // the query head that column `col` is
     int seq;
     const int len = pg_len(a, row, seq);
     const int lo = split * a.chunk, hi = min(len, lo + a.chunk);
+    // the table's entry for the slot that is key `col` of each tile (asked for without waiting for the length)
+    auto entry = [&](int b, int *pg) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int s = lo + b * KEYS + 16 * t + col;
+            pg[t] = s < a.max_len ? a.c.table[(size_t)seq * a.c.max_pages + (s >> a.c.page_shift)] : -1;
+        }
+    };
+    int pg[NT], nx[NT];
+    entry(wave, pg);
+    entry(wave + ATT_WAVES, nx);
     if (lo >= hi) {
         if (a.splits == 1)                                   // nothing to attend to: zeros
             for (int i = threadIdx.x; i < gn * HD; i += 64 * ATT_WAVES) {
@@ -204,7 +222,7 @@ template <int HD, bool QB, bool CB> __global__ __launch_bounds__(64 * ATT_WAVES)
     // queries: column `col` of the tile, the reduction elements that this lane's pieces of a key hold
     uint4 qr[QN];
     {
-        const long long at = (long long)row * a.q_stride + (long long)(head0 + (col < gn ? col : 0)) * HD;
+        const long long at = (long long)row * a.q_stride + (long long)(head0 + (qcol < gn ? qcol : 0)) * HD;
 #pragma unroll
         for (int j = 0; j < KQ; ++j) {
             if (CB) {
@@ -238,20 +256,18 @@ template <int HD, bool QB, bool CB> __global__ __launch_bounds__(64 * ATT_WAVES)
                 }
             }
         }
-        if (col >= gn)
+        if (qcol >= gn)
 #pragma unroll
             for (int j = 0; j < QN; ++j) qr[j] = make_uint4(0, 0, 0, 0);
     }
 
     const char *kb = a.c.k + (long long)kvh * a.c.stride_head + 16 * grp, *vb = a.c.v + (long long)kvh * a.c.stride_head;
-    // page of the slot that is key `col` of each tile; -1: past the end, or without a page.  What is read for such a
-    // slot lies in page 0 and does not count: its score becomes -inf and its value zero (it may hold a NaN).
-    auto look = [&](int b, int *pg) {
+    // entries to pages; -1: past the end, or without a page.  What is read for such a slot lies in page 0 and does
+    // not count: its score becomes -inf and its value zero (it may hold a NaN).
+    auto pages = [&](int b, int *pg) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int s = lo + b * KEYS + 16 * t + col;
-            pg[t] = s < hi ? pg_page(a.c, seq, s) : -1;
-        }
+        for (int t = 0; t < NT; ++t)
+            if (lo + b * KEYS + 16 * t + col >= hi || (unsigned)pg[t] >= (unsigned)a.c.n_pages) pg[t] = -1;
     };
     auto load_k = [&](int b, const int *pg, Tile &x) {
 #pragma unroll
@@ -296,13 +312,12 @@ template <int HD, bool QB, bool CB> __global__ __launch_bounds__(64 * ATT_WAVES)
     float m = -INFINITY, l = 0.0f;                           // of head `col`: m the same in its four lanes, l each lane's own share
     const int blocks = (hi - lo + KEYS - 1) / KEYS;
     Tile x;
-    int pg[NT], nx[NT];
     int b = wave;
     if (b < blocks) {
-        look(b, pg);
+        pages(b, pg);
         load_k(b, pg, x);
         load_v(b, pg, x);
-        look(b + ATT_WAVES, nx);
+        pages(b + ATT_WAVES, nx);
     }
     for (; b < blocks; b += ATT_WAVES) {
         pg_f4 s[NT];
@@ -374,63 +389,64 @@ template <int HD, bool QB, bool CB> __global__ __launch_bounds__(64 * ATT_WAVES)
                 for (int e = 0; e < NE; ++e) {
                     const uint32_t w = x.v[t][r][CB ? e / 2 : e];
                     const float f = __uint_as_float(!CB ? w : e % 2 ? w & 0xffff0000u : w << 16);
-                    acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(f, p[t][r], acc[e], 0, 0, 0);
+                    if (FEW) acc[e] = __builtin_amdgcn_mfma_f32_4x4x1f32(f, p[t][r], acc[e], 0, 0, 0);
+                    else acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(f, p[t][r], acc[e], 0, 0, 0);
                 }
         if (more) {
             load_v(b + ATT_WAVES, nx, x);
 #pragma unroll
             for (int t = 0; t < NT; ++t) pg[t] = nx[t];
-            look(b + 2 * ATT_WAVES, nx);
+            entry(b + 2 * ATT_WAVES, nx);
+            pages(b + 2 * ATT_WAVES, nx);
         }
     }
 
-    // the waves' shares joined: every wave's output in LDS, 16 dims of a head per element index, summed in wave order
+    // the waves' shares joined in LDS and summed in a fixed order, up to 8 elements of each lane (128 dims) at a time.
+    // Result row m of element e is dim m * ce + e - e0 of that part; with few heads a wave's four lane groups hold
+    // sums over keys of their own, which are shares like those of the waves.
+    constexpr int HEADS = FEW ? 4 : 16, SHARES = 16 * ATT_WAVES / HEADS;
     l += __shfl_xor(l, 16, WAVE);
     l += __shfl_xor(l, 32, WAVE);
-    if (grp == 0) { sm_m[wave][col] = m; sm_l[wave][col] = l; }
-    const int head = threadIdx.x >> 4, part = threadIdx.x & 15;
+    if (lane < HEADS) { sm_m[wave][lane] = m; sm_l[wave][lane] = l; }
+    const int row0 = FEW ? 4 * ((lane >> 2) & 3) : 4 * grp;
+    const int mine = FEW ? (4 * wave + grp) * HEADS + qcol : wave * HEADS + col;
     float M = -INFINITY, L = 0.0f, wt[ATT_WAVES];
 #pragma unroll
     for (int e0 = 0; e0 < NE; e0 += CB && NE - e0 >= 8 ? 8 : 4) {
-        const int ce = CB && NE - e0 >= 8 ? 8 : 4;
+        const int ce = CB && NE - e0 >= 8 ? 8 : 4;           // 16 * ce dims of every head: 4 a thread, in rounds
         if (e0) __syncthreads();
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int e = 0; e < ce; e += 4)
-                *(float4 *)&sm_o[wave][col][(4 * grp + r) * ce + e] =
+                *(float4 *)&sm_o[mine][(row0 + r) * ce + e] =
                     make_float4(acc[e0 + e][r], acc[e0 + e + 1][r], acc[e0 + e + 2][r], acc[e0 + e + 3][r]);
         __syncthreads();
-        if (e0 == 0) {
+#pragma unroll
+        for (int i = 0; i < (HEADS * 4 * ce + 64 * ATT_WAVES - 1) / (64 * ATT_WAVES); ++i) {
+            const int at = i * 64 * ATT_WAVES + (int)threadIdx.x, head = at / (4 * ce), d = at % (4 * ce) * 4;
+            if (head >= gn) continue;
+            M = -INFINITY; L = 0.0f;
 #pragma unroll
             for (int w = 0; w < ATT_WAVES; ++w) M = fmaxf(M, sm_m[w][head]);
             const float ms = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-            for (int w = 0; w < ATT_WAVES; ++w) { wt[w] = __builtin_amdgcn_exp2f(sm_m[w][head] - ms); L += wt[w] * sm_l[w][head]; }
-        }
-        float o[8];
+            for (int w = 0; w < ATT_WAVES; ++w) { wt[w] = __builtin_amdgcn_exp2f(sm_m[w][head] - ms); L = fmaf(wt[w], sm_l[w][head], L); }
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int e = 0; e < ce; ++e) o[e] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < ATT_WAVES; ++w)
-#pragma unroll
-            for (int e = 0; e < ce; ++e) o[e] = fmaf(wt[w], sm_o[w][head][part * ce + e], o[e]);
-        if (head < gn) {
-            const int d = 16 * e0 + part * ce;
+            for (int k = 0; k < SHARES; ++k) {
+                const float4 x = *(const float4 *)&sm_o[k * HEADS + head][d];
+                const float w = wt[FEW ? k / 4 : k];
+                o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+            }
             if (a.splits == 1) {
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                const long long at = (long long)row * a.out_stride + (long long)(head0 + head) * HD + d;
-#pragma unroll
-                for (int e = 0; e < ce; e += 4) {
-                    float y[4] = {o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
-                    pg_put_n<QB, 4>(a.out, at + e, y);
-                }
+                float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+                pg_put_n<QB, 4>(a.out, (long long)row * a.out_stride + (long long)(head0 + head) * HD + 16 * e0 + d, y);
             } else {
                 const size_t slot = ((size_t)row * a.heads + head0 + head) * a.splits + split;
-#pragma unroll
-                for (int e = 0; e < ce; e += 4)
-                    *(float4 *)(a.part_o + slot * HD + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                if (e0 == 0 && part == 0) *(float2 *)(a.part_ml + 2 * slot) = make_float2(M, L);
+                *(float4 *)(a.part_o + slot * HD + 16 * e0 + d) = o;
+                if (e0 == 0 && d == 0) *(float2 *)(a.part_ml + 2 * slot) = make_float2(M, L);
             }
         }
     }

@@ -66,7 +66,8 @@ PagedView view(const hipdec_paged_cache &c) {
 struct Split { int chunk, splits; };
 Split split_of(uint64_t n_rows, uint32_t kv_heads, uint32_t g, uint64_t max_len) {
     const uint64_t units = n_rows * kv_heads * ((g + 15) / 16), steps = (max_len + 127) / 128;
-    uint64_t per = (units * steps + 4 * kCus - 1) / (4 * kCus);
+    const uint64_t want = units ? (2 * kCus + units - 1) / units : 1;
+    uint64_t per = (steps + want - 1) / want;
     if (per < 1) per = 1;
     if (per > 8) per = 8;
     if (steps <= per) return Split{(int)(steps ? steps : 1) * 128, 1};
@@ -74,7 +75,8 @@ Split split_of(uint64_t n_rows, uint32_t kv_heads, uint32_t g, uint64_t max_len)
 }
 
 template <int HD, bool QB, bool CB> void go_attention(const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
-    hipLaunchKernelGGL((k_attn_paged<HD, QB, CB>), dim3(grid), dim3(64 * ATT_WAVES), 0, s, a);
+    if (a.g <= 4) hipLaunchKernelGGL((k_attn_paged<HD, QB, CB, true>), dim3(grid), dim3(64 * ATT_WAVES), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_paged<HD, QB, CB, false>), dim3(grid), dim3(64 * ATT_WAVES), 0, s, a);
     if (joins) hipLaunchKernelGGL((k_attn_paged_join<HD, QB>), dim3(joins), dim3(256), 0, s, a);
 }
 template <int HD> void go_attention(bool qb, bool cb, const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
