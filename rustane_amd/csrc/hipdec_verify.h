@@ -14,10 +14,10 @@
 #include "hipdec_common.h"
 
 #define VF_THREADS 256
-#define VF_PER 16                                            // logits per thread
-#define VF_CHUNK (VF_THREADS * VF_PER)
+#define VF_WAVES (VF_THREADS / WAVE)
 
-struct VfStat { double sum; float top; uint32_t arg; };      // of one chunk of one row: max z, its first index, sum exp((z - max) / T)
+struct VfStat { double sum; float top; uint32_t arg; };      // of one chunk of one row: max logit, its first index, sum of weights
+struct VfPlace { double inv; float top; int kept; };         // where a sequence's next token is drawn: 1 / the row's sum (0: nothing to draw), its maximum
 
 struct VerifyArgs {
     const void *logits;
@@ -25,10 +25,11 @@ struct VerifyArgs {
     const int *drafts, *n_drafts;
     const float *probs, *u;
     int n_seqs, max_drafts, vocab, chunks;
-    double inv_t;                                            // 0: greedy
-    float softcap;
+    double k;                                                // log2(e) / T; 0: greedy
+    double cap, cap_k;                                       // soft cap (0: none) and 2 log2(e) / cap
     VfStat *stats;                                           // [row][chunk]
     double *sums;                                            // [seq][chunk] of max(p - q, 0)
+    VfPlace *places;                                         // [seq]
     uint32_t *tokens;
     int *accepted;
 };
@@ -41,13 +42,43 @@ template <bool B16> __device__ __forceinline__ float vf_logit(const VerifyArgs &
     const float x = B16 ? bf16_to_f32(((const uint16_t *)a.logits)[at]) : ((const float *)a.logits)[at];
     return x == x ? x : -INFINITY;                           // a NaN is no possible token
 }
-__device__ __forceinline__ double vf_capped(const VerifyArgs &a, float x) {
-    return a.softcap > 0.0f ? (double)a.softcap * tanh((double)x / (double)a.softcap) : (double)x;
+
+// 2^y for y <= 1022: y = n + f with |f| <= 1/2, the series of 2^f = e^(f ln 2) up to its 12th power (the rest is below
+// 0.3466^13 / 13! = 2e-16 of it), scaled by 2^n.  A third of the instructions of the library's exp, which these
+// kernels are bound by: the largest case 295 -> 196 us.
+__device__ __forceinline__ double vf_exp2(double y) {
+    y = fmax(y, -1100.0);
+    const double n = rint(y), f = y - n;
+    double p = 2.5678435993488205e-11;                       // (ln 2)^12 / 12!
+    p = fma(p, f, 4.4455382718708116e-10);
+    p = fma(p, f, 7.0549116208011238e-09);
+    p = fma(p, f, 1.0178086009239699e-07);
+    p = fma(p, f, 1.3215486790144307e-06);
+    p = fma(p, f, 1.5252733804059841e-05);
+    p = fma(p, f, 1.5403530393381608e-04);
+    p = fma(p, f, 1.3333558146428443e-03);
+    p = fma(p, f, 9.6181291076284772e-03);
+    p = fma(p, f, 5.5504108664821580e-02);
+    p = fma(p, f, 2.4022650695910072e-01);
+    p = fma(p, f, 6.9314718055994531e-01);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n);
 }
-// exp((z - max z) / T); the maximum's own weight is 1 also where it is infinite, an impossible token's is 0
-__device__ __forceinline__ double vf_weight(const VerifyArgs &a, float x, float top) {
-    if (x == top) return x == -INFINITY ? 0.0 : 1.0;
-    return x == -INFINITY ? 0.0 : exp((vf_capped(a, x) - vf_capped(a, top)) * a.inv_t);
+// softcap(x) = cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1): off by 1e-15 of the cap, absolutely, which is what
+// the exponent behind it needs
+__device__ __forceinline__ double vf_capped(const VerifyArgs &a, float x) {
+    if (a.cap == 0.0) return (double)x;
+    const double d = vf_exp2(fmin((double)x * a.cap_k, 1000.0)) + 1.0;
+    double r = __builtin_amdgcn_rcp(d);                      // 1 / d by Newton's method: each step squares the error
+    r = fma(r, fma(-d, r, 1.0), r);
+    r = fma(r, fma(-d, r, 1.0), r);
+    return fma(-2.0 * a.cap, r, a.cap);
+}
+// exp((z - max z) / T); the maximum's own weight is 1 also where it is infinite, an impossible token's is 0.
+// ztop = vf_capped(top)
+__device__ __forceinline__ double vf_weight(const VerifyArgs &a, float x, float top, double ztop) {
+    if (x == -INFINITY) return 0.0;
+    return x == top ? 1.0 : vf_exp2((vf_capped(a, x) - ztop) * a.k);
 }
 __device__ __forceinline__ double vf_wave_sum(double v) {
 #pragma unroll
@@ -55,33 +86,38 @@ __device__ __forceinline__ double vf_wave_sum(double v) {
     return v;
 }
 
-// The statistics of every row that a sequence's drafts reach, one workgroup per chunk.
-template <bool B16> __global__ __launch_bounds__(VF_THREADS) void k_verify_stats(VerifyArgs a) {
-    __shared__ float st[4];
-    __shared__ uint32_t si[4];
-    __shared__ double ss[4];
+// The statistics of every row that a sequence's drafts reach, one workgroup per chunk of PER logits a thread.
+template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_stats(VerifyArgs a) {
+    __shared__ float st[VF_WAVES];
+    __shared__ uint32_t si[VF_WAVES];
+    __shared__ double ss[VF_WAVES];
     const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks;
     const int s = row / (a.max_drafts + 1);
-    if (row - s * (a.max_drafts + 1) > vf_drafts(a, s)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    float x[VF_PER];
+    float x[PER];
+    const bool unused = row - s * (a.max_drafts + 1) > vf_drafts(a, s);
+    if (PER > 4 && unused) return;                           // (few logits are asked for without waiting for the draft's length)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = (chunk * PER + i) * VF_THREADS + tid;
+        x[i] = at < a.vocab ? vf_logit<B16>(a, row, at) : -INFINITY;
+    }
+    if (unused) return;
     float top = -INFINITY; uint32_t arg = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < VF_PER; ++i) {
-        const int at = chunk * VF_CHUNK + i * VF_THREADS + tid;
-        x[i] = at < a.vocab ? vf_logit<B16>(a, row, at) : -INFINITY;
-        if (x[i] > top) { top = x[i]; arg = (uint32_t)at; }
-    }
+    for (int i = 0; i < PER; ++i)
+        if (x[i] > top) { top = x[i]; arg = (uint32_t)((chunk * PER + i) * VF_THREADS + tid); }
     wave_argbest(top, arg);
     if (lane == 0) { st[wave] = top; si[wave] = arg; }
     __syncthreads();
     top = st[0]; arg = si[0];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) if (better(st[w], si[w], top, arg)) { top = st[w]; arg = si[w]; }
+    for (int w = 1; w < VF_WAVES; ++w) if (better(st[w], si[w], top, arg)) { top = st[w]; arg = si[w]; }
     double sum = 0.0;
-    if (a.inv_t > 0.0) {
+    if (a.k > 0.0) {
+        const double ztop = vf_capped(a, top);
 #pragma unroll
-        for (int i = 0; i < VF_PER; ++i) sum += vf_weight(a, x[i], top);
+        for (int i = 0; i < PER; ++i) sum += vf_weight(a, x[i], top, ztop);
         sum = vf_wave_sum(sum);
         if (lane == 0) ss[wave] = sum;
         __syncthreads();
@@ -90,145 +126,158 @@ template <bool B16> __global__ __launch_bounds__(VF_THREADS) void k_verify_stats
     if (tid == 0) a.stats[(size_t)row * a.chunks + chunk] = VfStat{sum, top, arg};
 }
 
-// One row's maximum, its first index, and the sum over the whole row (a wave, every lane with the result).
-__device__ __forceinline__ void vf_row(const VerifyArgs &a, long long row, float &top, uint32_t &arg, double &sum) {
-    const VfStat *st = a.stats + (size_t)row * a.chunks;
-    top = -INFINITY; arg = 0xffffffffu;
-    for (int i = threadIdx.x & 63; i < a.chunks; i += WAVE)
-        if (better(st[i].top, st[i].arg, top, arg)) { top = st[i].top; arg = st[i].arg; }
-    wave_argbest(top, arg);
-    sum = 0.0;
-    if (a.inv_t > 0.0) {
-        for (int i = threadIdx.x & 63; i < a.chunks; i += WAVE) sum += st[i].sum * vf_weight(a, st[i].top, top);
-        sum = vf_wave_sum(sum);
-    }
-}
-
-struct VfPlace { int kept, n; long long row; float top; uint32_t arg; double inv; };
-
-// How many drafts of sequence s are kept, and the row the next token is drawn from (every thread with the result).
-template <bool B16> __device__ __forceinline__ VfPlace vf_decide(const VerifyArgs &a, int s) {
-    __shared__ int first;                                    // the first draft that is not kept
-    const int n = vf_drafts(a, s), wave = threadIdx.x >> 6, K = a.max_drafts;
-    if (threadIdx.x == 0) first = n;
+// The decision, by every workgroup of the sequence for itself (a wave per draft, all of them at once up to four), then
+// the workgroup's chunk of max(p - q, 0) where a draft was not kept.  The first chunk's workgroup writes what is known
+// by now: the kept drafts and, where T = 0 or nothing is possible, the next token.
+template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_decide(VerifyArgs a) {
+    __shared__ double s_inv[256], ss[VF_WAVES];              // of each row (max_drafts <= 255)
+    __shared__ float s_top[256];
+    __shared__ uint32_t s_arg[256];
+    __shared__ int s_kept;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.max_drafts;
+    const int part = a.k > 0.0 ? (int)(blockIdx.x % a.chunks) : 0, s = a.k > 0.0 ? (int)(blockIdx.x / a.chunks) : (int)blockIdx.x;
+    const int n = vf_drafts(a, s);
+    if (tid == 0) s_kept = n;
     __syncthreads();
-    for (int i = wave; i < n; i += VF_THREADS / WAVE) {
+    for (int i = wave; i <= n; i += VF_WAVES) {
         const long long row = (long long)s * (K + 1) + i;
-        float top; uint32_t arg; double sum;
-        vf_row(a, row, top, arg, sum);
-        const int d = a.drafts[(size_t)s * K + i];
-        bool keep = false;
-        if ((unsigned)d < (unsigned)a.vocab) {
-            if (a.inv_t > 0.0) {
-                const double p = sum > 0.0 ? vf_weight(a, vf_logit<B16>(a, row, d), top) / sum : 0.0;
-                const double q = a.probs ? (double)a.probs[((long long)s * K + i) * a.prob_stride + d] : 1.0;
-                keep = (double)a.u[(size_t)s * (K + 1) + i] * q < p;
-            } else {
-                keep = (uint32_t)d == arg;
-            }
+        const int d = i < n ? a.drafts[(size_t)s * K + i] : -1;
+        const bool real = (unsigned)d < (unsigned)a.vocab;
+        const float x = real ? vf_logit<B16>(a, row, d) : -INFINITY;
+        const double q = real && a.k > 0.0 && a.probs ? (double)a.probs[((long long)s * K + i) * a.prob_stride + d] : 1.0;
+        const double u = a.k > 0.0 && i < n ? (double)a.u[(size_t)s * (K + 1) + i] : 0.0;
+        const VfStat *st = a.stats + (size_t)row * a.chunks;
+        float top = -INFINITY; uint32_t arg = 0xffffffffu;
+        VfStat mine[4];                                      // at most 256 chunks
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine[j] = lane + 64 * j < a.chunks ? st[lane + 64 * j] : VfStat{0.0, -INFINITY, 0xffffffffu};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (better(mine[j].top, mine[j].arg, top, arg)) { top = mine[j].top; arg = mine[j].arg; }
+        wave_argbest(top, arg);
+        double sum = 0.0, ztop = 0.0;
+        if (a.k > 0.0) {
+            ztop = vf_capped(a, top);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (64 * j < a.chunks) sum += mine[j].sum * vf_weight(a, mine[j].top, top, ztop);
+            sum = vf_wave_sum(sum);
         }
-        if (!keep && (threadIdx.x & 63) == 0) atomicMin(&first, i);
+        const double inv = sum > 0.0 ? 1.0 / sum : 0.0;
+        const bool keep = real && (a.k > 0.0 ? u * q < vf_weight(a, x, top, ztop) * inv : (uint32_t)d == arg);
+        if (lane == 0) {
+            s_inv[i] = inv; s_top[i] = top; s_arg[i] = arg;
+            if (i < n && !keep) atomicMin(&s_kept, i);
+        }
     }
     __syncthreads();
-    VfPlace at;
-    at.n = n; at.kept = first;
-    at.row = (long long)s * (K + 1) + at.kept;
-    double sum;
-    vf_row(a, at.row, at.top, at.arg, sum);
-    at.inv = sum > 0.0 ? 1.0 / sum : 0.0;
-    return at;
-}
-
-// The weight of token i in what the next token is drawn from; `rest`: the part of the target the draft did not cover.
-template <bool B16> __device__ __forceinline__ double vf_mass(const VerifyArgs &a, const VfPlace &at, int s, int i, bool rest) {
-    const double p = vf_weight(a, vf_logit<B16>(a, at.row, i), at.top) * at.inv;
-    if (!rest) return p;
-    const long long d = (long long)s * a.max_drafts + at.kept;
-    const double q = a.probs ? (double)a.probs[d * a.prob_stride + i] : a.drafts[d] == i ? 1.0 : 0.0;
-    return fmax(p - q, 0.0);                                 // (a NaN in q leaves 0)
-}
-
-// Chunk sums of max(p - q, 0) at a sequence's first draft that is not kept.
-template <bool B16> __global__ __launch_bounds__(VF_THREADS) void k_verify_sums(VerifyArgs a) {
-    __shared__ double ss[4];
-    const int chunk = blockIdx.x % a.chunks, s = blockIdx.x / a.chunks;
-    const VfPlace at = vf_decide<B16>(a, s);
-    if (at.kept == at.n || !(a.inv_t > 0.0)) return;         // the statistics hold the target's own sums
+    const int kept = s_kept;
+    const double inv = s_inv[kept];
+    const float top = s_top[kept];
+    if (part == 0) {
+        uint32_t *out = a.tokens + (size_t)s * (K + 1);
+        const bool known = !(a.k > 0.0) || inv == 0.0;       // (the index of a row without a possible token is 0xffffffff)
+        for (int i = tid; i <= K; i += VF_THREADS)
+            if (i != kept || known) out[i] = i < kept ? (uint32_t)a.drafts[(size_t)s * K + i] : i == kept ? s_arg[kept] : 0xffffffffu;
+        if (tid == 0) { a.accepted[s] = kept; a.places[s] = VfPlace{inv, top, kept}; }
+    }
+    if (kept == n || !(a.k > 0.0)) return;                   // behind the last draft the statistics hold the sums
+    const long long row = (long long)s * (K + 1) + kept, dr = (long long)s * K + kept;
+    const double ztop = vf_capped(a, top);
+    float x[PER], q[PER];
+    const int d = a.drafts[dr];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = (part * PER + j) * VF_THREADS + tid;
+        x[j] = i < a.vocab ? vf_logit<B16>(a, row, i) : -INFINITY;
+        q[j] = i < a.vocab ? a.probs ? a.probs[dr * a.prob_stride + i] : d == i ? 1.0f : 0.0f : 0.0f;
+    }
     double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < VF_PER; ++j) {
-        const int i = chunk * VF_CHUNK + j * VF_THREADS + (int)threadIdx.x;
-        if (i < a.vocab) sum += vf_mass<B16>(a, at, s, i, true);
-    }
+    for (int j = 0; j < PER; ++j) sum += fmax(vf_weight(a, x[j], top, ztop) * inv - (double)q[j], 0.0);   // (a NaN in q leaves 0)
     sum = vf_wave_sum(sum);
-    if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = sum;
+    if (lane == 0) ss[wave] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) a.sums[(size_t)s * a.chunks + chunk] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+    if (tid == 0) a.sums[(size_t)s * a.chunks + part] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
 }
 
-// running sum over the lanes of a wave, the lane's own term included
-__device__ __forceinline__ double vf_wave_scan(double v) {
+// sum over the threads before this one and this one, and the whole (VF_WAVES values of LDS)
+__device__ __forceinline__ double vf_scan(double v, double *waves, double &before, double &whole) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double run = v;
 #pragma unroll
     for (int o = 1; o < WAVE; o <<= 1) {
-        const double w = __shfl_up(v, o, WAVE);
-        if ((int)(threadIdx.x & 63) >= o) v += w;
+        const double w = __shfl_up(run, o, WAVE);
+        if (lane >= o) run += w;
     }
-    return v;
+    if (lane == 63) waves[wave] = run;
+    const double up = __shfl_up(run, 1, WAVE);
+    __syncthreads();
+    double base = 0.0;
+    whole = 0.0;
+#pragma unroll
+    for (int k = 0; k < VF_WAVES; ++k) { if (k < wave) base += waves[k]; whole += waves[k]; }
+    before = base + (lane ? up : 0.0);
+    return base + run;
 }
 
-// The draw: the chunk where the running sum passes the border, then the token inside it.
-template <bool B16> __global__ __launch_bounds__(VF_THREADS) void k_verify_draw(VerifyArgs a) {
-    __shared__ double part[VF_THREADS / WAVE], left;
-    __shared__ int chunk, from_rest, hit, last;
-    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.max_drafts;
-    const VfPlace at = vf_decide<B16>(a, s);
-    for (int i = tid; i <= K; i += VF_THREADS)
-        if (i != at.kept) a.tokens[(size_t)s * (K + 1) + i] = i < at.kept ? (uint32_t)a.drafts[(size_t)s * K + i] : 0xffffffffu;
-    if (tid == 0) a.accepted[s] = at.kept;
-    uint32_t *out = a.tokens + (size_t)s * (K + 1) + at.kept;
-    if (!(a.inv_t > 0.0) || at.inv == 0.0) {                 // greedy; or no possible token at all (arg is 0xffffffff then)
-        if (tid == 0) *out = at.arg;
-        return;
+// The draw: the chunk where the running sum passes the border (a thread per chunk), then the token inside it.
+template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_draw(VerifyArgs a) {
+    __shared__ double w1[VF_WAVES], w2[VF_WAVES], left;
+    __shared__ int hit_chunk, last_chunk, some, hit, last;
+    const int s = blockIdx.x, tid = threadIdx.x, K = a.max_drafts;
+    const int n = vf_drafts(a, s);
+    const VfPlace at = a.places[s];
+    const float u = a.u[(size_t)s * (K + 1) + K];
+    double mine = tid < a.chunks && at.kept < n ? a.sums[(size_t)s * a.chunks + tid] : 0.0;
+    if (at.inv == 0.0) return;                               // no possible token: already written
+    const long long row = (long long)s * (K + 1) + at.kept, dr = (long long)s * K + at.kept;
+    const double ztop = vf_capped(a, at.top);
+    if (tid == 0) { hit_chunk = 0x7fffffff; last_chunk = -1; some = 0; hit = 0x7fffffff; last = -1; }
+    __syncthreads();
+    if (mine > 0.0) some = 1;
+    __syncthreads();
+    // all drafts kept, or the draft's distribution covers the target's everywhere: the target's own
+    const bool rest = some != 0;
+    if (!rest) {
+        const VfStat st = tid < a.chunks ? a.stats[(size_t)row * a.chunks + tid] : VfStat{0.0, -INFINITY, 0u};
+        mine = st.sum * vf_weight(a, st.top, at.top, ztop) * at.inv;
     }
-    if (wave == 0) {                                         // at most 64 chunks: one a lane
-        bool rest = at.kept < at.n;
-        double mine = rest && lane < a.chunks ? a.sums[(size_t)s * a.chunks + lane] : 0.0;
-        // all drafts kept, or the draft's distribution covers the target's everywhere: the target's own
-        if (!rest || !__any(mine > 0.0)) {
-            rest = false;
-            const VfStat *st = a.stats + (size_t)at.row * a.chunks;
-            mine = lane < a.chunks ? st[lane].sum * vf_weight(a, st[lane].top, at.top) * at.inv : 0.0;
-        }
-        const double run = vf_wave_scan(mine), border = (double)a.u[(size_t)s * (K + 1) + K] * __shfl(run, 63, WAVE);
-        const uint64_t some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && run > border);
-        // (no chunk passes the border where the random number is 1 or the sums round down: the last one with any weight)
-        const int c = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)some);
-        const double before = __shfl_up(run, 1, WAVE);
-        if (lane == c) { chunk = c; from_rest = rest; left = border - (lane ? before : 0.0); hit = 0x7fffffff; last = 0; }
+    double before, whole;
+    const double run = vf_scan(mine, w1, before, whole), border = (double)u * whole;
+    // (no chunk passes the border where the random number is 1 or the sums round down: the last one with any weight)
+    if (mine > 0.0) {
+        atomicMax(&last_chunk, tid);
+        if (run > border) atomicMin(&hit_chunk, tid);
     }
     __syncthreads();
-    const int i0 = chunk * VF_CHUNK + tid * VF_PER;          // in index order
-    double w[VF_PER], mine = 0.0;
+    const int chunk = hit_chunk != 0x7fffffff ? hit_chunk : last_chunk;
+    if (tid == chunk) left = border - before;
+    const int i0 = (chunk * VF_THREADS + tid) * PER;         // in index order
+    float x[PER], q[PER];
+    const int d = rest ? a.drafts[dr] : -1;
 #pragma unroll
-    for (int j = 0; j < VF_PER; ++j) {
-        w[j] = i0 + j < a.vocab ? vf_mass<B16>(a, at, s, i0 + j, from_rest) : 0.0;
+    for (int j = 0; j < PER; ++j) {
+        const int i = i0 + j;
+        x[j] = i < a.vocab ? vf_logit<B16>(a, row, i) : -INFINITY;
+        q[j] = i < a.vocab && rest ? a.probs ? a.probs[dr * a.prob_stride + i] : d == i ? 1.0f : 0.0f : 0.0f;
+    }
+    double w[PER];
+    mine = 0.0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const double p = vf_weight(a, x[j], at.top, ztop) * at.inv;
+        w[j] = rest ? fmax(p - (double)q[j], 0.0) : p;
         mine += w[j];
     }
-    const double run = vf_wave_scan(mine);
-    if (lane == 63) part[wave] = run;
-    __syncthreads();
-    const double before = __shfl_up(run, 1, WAVE);
-    double r = lane ? before : 0.0;
+    double r;
+    vf_scan(mine, w2, r, whole);                             // (its barrier also publishes `left`)
+    int my_hit = 0x7fffffff, my_last = -1;
 #pragma unroll
-    for (int k = 0; k < VF_THREADS / WAVE; ++k) if (k < wave) r += part[k];
-    int mine_hit = 0x7fffffff, mine_last = -1;
-#pragma unroll
-    for (int j = 0; j < VF_PER; ++j) {
+    for (int j = 0; j < PER; ++j) {
         r += w[j];
-        if (w[j] > 0.0) { mine_last = i0 + j; if (r > left) mine_hit = min(mine_hit, i0 + j); }
+        if (w[j] > 0.0) { my_last = i0 + j; if (r > left) my_hit = min(my_hit, i0 + j); }
     }
-    if (mine_hit != 0x7fffffff) atomicMin(&hit, mine_hit);
-    if (mine_last >= 0) atomicMax(&last, mine_last);
+    if (my_hit != 0x7fffffff) atomicMin(&hit, my_hit);
+    if (my_last >= 0) atomicMax(&last, my_last);
     __syncthreads();
-    if (tid == 0) *out = (uint32_t)(hit != 0x7fffffff ? hit : last);
+    if (tid == 0) a.tokens[(size_t)s * (K + 1) + at.kept] = (uint32_t)(hit != 0x7fffffff ? hit : last);
 }

@@ -89,13 +89,22 @@ template <bool RB, bool CB> void go_rope(const RopeArgs &a, bool wide, unsigned 
     else hipLaunchKernelGGL((k_rope_append<RB, CB, 1>), dim3(grid), dim3(ROPE_THREADS), 0, s, a);
 }
 
-uint64_t chunks_of(uint32_t vocab) { return (vocab + VF_CHUNK - 1) / VF_CHUNK; }
+// Logits of a row per workgroup: 1024 where that makes few workgroups (the draw of one sequence is latency), else 4096
+// (fewer reductions, and less of the statistics to read back).  At most 256 chunks: a thread each.
+struct Chunks { int per, n; };
+Chunks chunks_of(uint64_t rows, uint32_t vocab) {
+    const int per = rows * vocab <= (uint64_t)16 * kCus * 1024 ? 4 : 16;
+    return Chunks{per, (int)((vocab + per * VF_THREADS - 1) / (per * VF_THREADS))};
+}
+uint64_t verify_bytes(uint64_t n_seqs, uint32_t max_drafts, int chunks) {
+    return n_seqs * ((max_drafts + 1) * chunks * sizeof(VfStat) + chunks * sizeof(double) + sizeof(VfPlace));
+}
 
-template <bool B16> void go_verify(const VerifyArgs &a, bool rest, hipStream_t s) {
-    const unsigned rows = (unsigned)a.n_seqs * (a.max_drafts + 1);
-    hipLaunchKernelGGL(k_verify_stats<B16>, dim3(rows * a.chunks), dim3(VF_THREADS), 0, s, a);
-    if (rest) hipLaunchKernelGGL(k_verify_sums<B16>, dim3((unsigned)a.n_seqs * a.chunks), dim3(VF_THREADS), 0, s, a);
-    hipLaunchKernelGGL(k_verify_draw<B16>, dim3((unsigned)a.n_seqs), dim3(VF_THREADS), 0, s, a);
+template <bool B16, int PER> void go_verify(const VerifyArgs &a, hipStream_t s) {
+    const unsigned rows = (unsigned)a.n_seqs * (a.max_drafts + 1), chunks = (unsigned)a.chunks, seqs = (unsigned)a.n_seqs;
+    hipLaunchKernelGGL((k_verify_stats<B16, PER>), dim3(rows * chunks), dim3(VF_THREADS), 0, s, a);
+    hipLaunchKernelGGL((k_verify_decide<B16, PER>), dim3(a.k > 0.0 ? seqs * chunks : seqs), dim3(VF_THREADS), 0, s, a);
+    if (a.k > 0.0) hipLaunchKernelGGL((k_verify_draw<B16, PER>), dim3(seqs), dim3(VF_THREADS), 0, s, a);
 }
 
 }  // namespace
@@ -231,7 +240,7 @@ int hipdec_verify_drafts_workspace(uint64_t n_seqs, uint32_t max_drafts, uint32_
     const char *me = "hipdec_verify_drafts_workspace";
     if (!out_bytes) return refuse(me, "null argument");
     if (max_drafts > kMaxDrafts || n_seqs > kMaxRows || !vocab || vocab > kMaxVocab) return refuse(me, "n_seqs, max_drafts or vocab out of range");
-    *out_bytes = n_seqs * chunks_of(vocab) * ((max_drafts + 1) * sizeof(VfStat) + sizeof(double));
+    *out_bytes = verify_bytes(n_seqs, max_drafts, chunks_of(n_seqs * (max_drafts + 1), vocab).n);
     return HIPDEC_OK;
 }
 
@@ -249,21 +258,24 @@ int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t wor
         return refuse(me, "n_seqs, max_drafts or vocab out of range");
     if (d->row_stride < d->vocab || (d->d_draft_probs && d->max_drafts && d->prob_stride < d->vocab))
         return refuse(me, "rows overlap: a stride is smaller than the vocabulary");
-    const uint64_t chunks = chunks_of(d->vocab), rows = d->n_seqs * (d->max_drafts + 1);
-    const uint64_t need = d->n_seqs * chunks * ((d->max_drafts + 1) * sizeof(VfStat) + sizeof(double));
+    const uint64_t rows = d->n_seqs * (d->max_drafts + 1);
+    const Chunks c = chunks_of(rows, d->vocab);
+    const uint64_t need = verify_bytes(d->n_seqs, d->max_drafts, c.n);
     if (!d_workspace || workspace_bytes < need || !aligned16(d_workspace))
         return refuse(me, "workspace missing, too small (hipdec_verify_drafts_workspace) or not 16-byte aligned");
-    if (rows * chunks > 0x7fffffffu) return refuse(me, "n_seqs * max_drafts * vocab out of range");
+    if (rows * c.n > 0x7fffffffu) return refuse(me, "n_seqs * max_drafts * vocab out of range");
     if ((bad = wrong_place({d->d_logits, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms, d->d_tokens, d->d_accepted,
                             d_workspace}, stream)))
         return refuse(me, bad);
     VfStat *st = (VfStat *)d_workspace;
+    VfPlace *places = (VfPlace *)(st + rows * c.n);
+    const double log2e = 1.4426950408889634074, cap = d->softcap > 0.0f ? d->softcap : 0.0;
     const VerifyArgs a{d->d_logits, d->row_stride, d->prob_stride, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms,
-                       (int)d->n_seqs, (int)d->max_drafts, (int)d->vocab, (int)chunks, greedy ? 0.0 : 1.0 / (double)d->temperature,
-                       d->softcap, st, (double *)(st + rows * chunks), d->d_tokens, d->d_accepted};
-    const bool rest = !greedy && d->max_drafts;
-    if (d->dtype == HIPDEC_ROWS_BF16) go_verify<true>(a, rest, (hipStream_t)stream);
-    else go_verify<false>(a, rest, (hipStream_t)stream);
+                       (int)d->n_seqs, (int)d->max_drafts, (int)d->vocab, c.n, greedy ? 0.0 : log2e / (double)d->temperature,
+                       cap, cap > 0.0 ? 2.0 * log2e / cap : 0.0, st, (double *)(places + d->n_seqs), places, d->d_tokens, d->d_accepted};
+    hipStream_t s = (hipStream_t)stream;
+    if (d->dtype == HIPDEC_ROWS_BF16) { if (c.per == 4) go_verify<true, 4>(a, s); else go_verify<true, 16>(a, s); }
+    else { if (c.per == 4) go_verify<false, 4>(a, s); else go_verify<false, 16>(a, s); }
     return launched(me);
 }
 
