@@ -43,31 +43,31 @@ template <bool B16> __device__ __forceinline__ float vf_logit(const VerifyArgs &
     return x == x ? x : -INFINITY;                           // a NaN is no possible token
 }
 
-// 2^y for y <= 1022: y = n + f with |f| <= 1/2, the series of 2^f = e^(f ln 2) up to its 12th power (the rest is below
-// 0.3466^13 / 13! = 2e-16 of it), scaled by 2^n.  A third of the instructions of the library's exp, which these
-// kernels are bound by: the largest case 295 -> 196 us.
+// 2^y for y <= 1022: y = n + f with |f| <= 1/2, the series of 2^f = e^(f ln 2) up to its 11th power (the rest is below
+// 0.3466^12 / 12! = 7e-15 of it), scaled by 2^n in the exponent's bits.  n is read off the last bits of y + 1.5 * 2^52.
+// Below 2^-1020 the result stays there.  (These kernels are bound by this: with the library's exp, and conversions
+// and ldexp, which run at a quarter of the rate, the largest case takes 295 us, so XX.)
 __device__ __forceinline__ double vf_exp2(double y) {
-    y = fmax(y, -1100.0);
-    const double n = rint(y), f = y - n;
-    double p = 2.5678435993488205e-11;                       // (ln 2)^12 / 12!
-    p = fma(p, f, 4.4455382718708116e-10);
-    p = fma(p, f, 7.0549116208011238e-09);
-    p = fma(p, f, 1.0178086009239699e-07);
-    p = fma(p, f, 1.3215486790144307e-06);
+    y = fmax(y, -1020.0);
+    const double whole = 6755399441055744.0, t = y + whole, f = y - (t - whole);
+    double p = 4.4455382718708116e-10;                       // (ln 2)^k / k!, k = 11 .. 0
+    p = fma(p, f, 7.054911620801123e-09);
+    p = fma(p, f, 1.01780860092397e-07);
+    p = fma(p, f, 1.321548679014431e-06);
     p = fma(p, f, 1.5252733804059841e-05);
-    p = fma(p, f, 1.5403530393381608e-04);
+    p = fma(p, f, 1.540353039338161e-04);
     p = fma(p, f, 1.3333558146428443e-03);
-    p = fma(p, f, 9.6181291076284772e-03);
-    p = fma(p, f, 5.5504108664821580e-02);
+    p = fma(p, f, 9.618129107628477e-03);
+    p = fma(p, f, 5.550410866482158e-02);
     p = fma(p, f, 2.4022650695910072e-01);
-    p = fma(p, f, 6.9314718055994531e-01);
+    p = fma(p, f, 6.931471805599453e-01);
     p = fma(p, f, 1.0);
-    return ldexp(p, (int)n);
+    return __hiloint2double(__double2hiint(p) + (int)((unsigned)__double2loint(t) << 20), __double2loint(p));
 }
 // softcap(x) = cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1): off by 1e-15 of the cap, absolutely, which is what
 // the exponent behind it needs
-__device__ __forceinline__ double vf_capped(const VerifyArgs &a, float x) {
-    if (a.cap == 0.0) return (double)x;
+template <bool CAP> __device__ __forceinline__ double vf_capped(const VerifyArgs &a, float x) {
+    if (!CAP) return (double)x;
     const double d = vf_exp2(fmin((double)x * a.cap_k, 1000.0)) + 1.0;
     double r = __builtin_amdgcn_rcp(d);                      // 1 / d by Newton's method: each step squares the error
     r = fma(r, fma(-d, r, 1.0), r);
@@ -75,10 +75,10 @@ __device__ __forceinline__ double vf_capped(const VerifyArgs &a, float x) {
     return fma(-2.0 * a.cap, r, a.cap);
 }
 // exp((z - max z) / T); the maximum's own weight is 1 also where it is infinite, an impossible token's is 0.
-// ztop = vf_capped(top)
-__device__ __forceinline__ double vf_weight(const VerifyArgs &a, float x, float top, double ztop) {
-    if (x == -INFINITY) return 0.0;
-    return x == top ? 1.0 : vf_exp2((vf_capped(a, x) - ztop) * a.k);
+// ztop = vf_capped(top).  (Selections, not branches: the exponentials of a thread's logits run side by side.)
+template <bool CAP> __device__ __forceinline__ double vf_weight(const VerifyArgs &a, float x, float top, double ztop) {
+    const double w = vf_exp2((vf_capped<CAP>(a, x) - ztop) * a.k);
+    return x == -INFINITY ? 0.0 : x == top ? 1.0 : w;
 }
 __device__ __forceinline__ double vf_wave_sum(double v) {
 #pragma unroll
@@ -87,7 +87,7 @@ __device__ __forceinline__ double vf_wave_sum(double v) {
 }
 
 // The statistics of every row that a sequence's drafts reach, one workgroup per chunk of PER logits a thread.
-template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_stats(VerifyArgs a) {
+template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_stats(VerifyArgs a) {
     __shared__ float st[VF_WAVES];
     __shared__ uint32_t si[VF_WAVES];
     __shared__ double ss[VF_WAVES];
@@ -115,9 +115,9 @@ template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_ver
     for (int w = 1; w < VF_WAVES; ++w) if (better(st[w], si[w], top, arg)) { top = st[w]; arg = si[w]; }
     double sum = 0.0;
     if (a.k > 0.0) {
-        const double ztop = vf_capped(a, top);
+        const double ztop = vf_capped<CAP>(a, top);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) sum += vf_weight(a, x[i], top, ztop);
+        for (int i = 0; i < PER; ++i) sum += vf_weight<CAP>(a, x[i], top, ztop);
         sum = vf_wave_sum(sum);
         if (lane == 0) ss[wave] = sum;
         __syncthreads();
@@ -129,7 +129,7 @@ template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_ver
 // The decision, by every workgroup of the sequence for itself (a wave per draft, all of them at once up to four), then
 // the workgroup's chunk of max(p - q, 0) where a draft was not kept.  The first chunk's workgroup writes what is known
 // by now: the kept drafts and, where T = 0 or nothing is possible, the next token.
-template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_decide(VerifyArgs a) {
+template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_decide(VerifyArgs a) {
     __shared__ double s_inv[256], ss[VF_WAVES];              // of each row (max_drafts <= 255)
     __shared__ float s_top[256];
     __shared__ uint32_t s_arg[256];
@@ -142,27 +142,27 @@ template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_ver
     for (int i = wave; i <= n; i += VF_WAVES) {
         const long long row = (long long)s * (K + 1) + i;
         const int d = i < n ? a.drafts[(size_t)s * K + i] : -1;
-        const bool real = (unsigned)d < (unsigned)a.vocab;
-        const float x = real ? vf_logit<B16>(a, row, d) : -INFINITY;
-        const double q = real && a.k > 0.0 && a.probs ? (double)a.probs[((long long)s * K + i) * a.prob_stride + d] : 1.0;
-        const double u = a.k > 0.0 && i < n ? (double)a.u[(size_t)s * (K + 1) + i] : 0.0;
         const VfStat *st = a.stats + (size_t)row * a.chunks;
         float top = -INFINITY; uint32_t arg = 0xffffffffu;
         VfStat mine[4];                                      // at most 256 chunks
 #pragma unroll
         for (int j = 0; j < 4; ++j) mine[j] = lane + 64 * j < a.chunks ? st[lane + 64 * j] : VfStat{0.0, -INFINITY, 0xffffffffu};
+        const bool real = (unsigned)d < (unsigned)a.vocab;
+        const float x = real ? vf_logit<B16>(a, row, d) : -INFINITY;
+        const double q = real && a.k > 0.0 && a.probs ? (double)a.probs[((long long)s * K + i) * a.prob_stride + d] : 1.0;
+        const double u = a.k > 0.0 && i < n ? (double)a.u[(size_t)s * (K + 1) + i] : 0.0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) if (better(mine[j].top, mine[j].arg, top, arg)) { top = mine[j].top; arg = mine[j].arg; }
         wave_argbest(top, arg);
         double sum = 0.0, ztop = 0.0;
         if (a.k > 0.0) {
-            ztop = vf_capped(a, top);
+            ztop = vf_capped<CAP>(a, top);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (64 * j < a.chunks) sum += mine[j].sum * vf_weight(a, mine[j].top, top, ztop);
+            for (int j = 0; j < 4; ++j) if (64 * j < a.chunks) sum += mine[j].sum * vf_weight<CAP>(a, mine[j].top, top, ztop);
             sum = vf_wave_sum(sum);
         }
         const double inv = sum > 0.0 ? 1.0 / sum : 0.0;
-        const bool keep = real && (a.k > 0.0 ? u * q < vf_weight(a, x, top, ztop) * inv : (uint32_t)d == arg);
+        const bool keep = real && (a.k > 0.0 ? u * q < vf_weight<CAP>(a, x, top, ztop) * inv : (uint32_t)d == arg);
         if (lane == 0) {
             s_inv[i] = inv; s_top[i] = top; s_arg[i] = arg;
             if (i < n && !keep) atomicMin(&s_kept, i);
@@ -181,7 +181,7 @@ template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_ver
     }
     if (kept == n || !(a.k > 0.0)) return;                   // behind the last draft the statistics hold the sums
     const long long row = (long long)s * (K + 1) + kept, dr = (long long)s * K + kept;
-    const double ztop = vf_capped(a, top);
+    const double ztop = vf_capped<CAP>(a, top);
     float x[PER], q[PER];
     const int d = a.drafts[dr];
 #pragma unroll
@@ -192,7 +192,7 @@ template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_ver
     }
     double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) sum += fmax(vf_weight(a, x[j], top, ztop) * inv - (double)q[j], 0.0);   // (a NaN in q leaves 0)
+    for (int j = 0; j < PER; ++j) sum += fmax(vf_weight<CAP>(a, x[j], top, ztop) * inv - (double)q[j], 0.0);   // (a NaN in q leaves 0)
     sum = vf_wave_sum(sum);
     if (lane == 0) ss[wave] = sum;
     __syncthreads();
@@ -220,17 +220,18 @@ __device__ __forceinline__ double vf_scan(double v, double *waves, double &befor
 }
 
 // The draw: the chunk where the running sum passes the border (a thread per chunk), then the token inside it.
-template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_draw(VerifyArgs a) {
+template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_draw(VerifyArgs a) {
     __shared__ double w1[VF_WAVES], w2[VF_WAVES], left;
     __shared__ int hit_chunk, last_chunk, some, hit, last;
     const int s = blockIdx.x, tid = threadIdx.x, K = a.max_drafts;
     const int n = vf_drafts(a, s);
     const VfPlace at = a.places[s];
     const float u = a.u[(size_t)s * (K + 1) + K];
-    double mine = tid < a.chunks && at.kept < n ? a.sums[(size_t)s * a.chunks + tid] : 0.0;
+    double mine = tid < a.chunks ? a.sums[(size_t)s * a.chunks + tid] : 0.0;
+    if (at.kept == n) mine = 0.0;                            // (nothing was written there)
     if (at.inv == 0.0) return;                               // no possible token: already written
     const long long row = (long long)s * (K + 1) + at.kept, dr = (long long)s * K + at.kept;
-    const double ztop = vf_capped(a, at.top);
+    const double ztop = vf_capped<CAP>(a, at.top);
     if (tid == 0) { hit_chunk = 0x7fffffff; last_chunk = -1; some = 0; hit = 0x7fffffff; last = -1; }
     __syncthreads();
     if (mine > 0.0) some = 1;
@@ -239,7 +240,7 @@ template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_ver
     const bool rest = some != 0;
     if (!rest) {
         const VfStat st = tid < a.chunks ? a.stats[(size_t)row * a.chunks + tid] : VfStat{0.0, -INFINITY, 0u};
-        mine = st.sum * vf_weight(a, st.top, at.top, ztop) * at.inv;
+        mine = st.sum * vf_weight<CAP>(a, st.top, at.top, ztop) * at.inv;
     }
     double before, whole;
     const double run = vf_scan(mine, w1, before, whole), border = (double)u * whole;
@@ -264,7 +265,7 @@ template <bool B16, int PER> __global__ __launch_bounds__(VF_THREADS) void k_ver
     mine = 0.0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const double p = vf_weight(a, x[j], at.top, ztop) * at.inv;
+        const double p = vf_weight<CAP>(a, x[j], at.top, ztop) * at.inv;
         w[j] = rest ? fmax(p - (double)q[j], 0.0) : p;
         mine += w[j];
     }

@@ -100,11 +100,16 @@ uint64_t verify_bytes(uint64_t n_seqs, uint32_t max_drafts, int chunks) {
     return n_seqs * ((max_drafts + 1) * chunks * sizeof(VfStat) + chunks * sizeof(double) + sizeof(VfPlace));
 }
 
-template <bool B16, int PER> void go_verify(const VerifyArgs &a, hipStream_t s) {
+template <bool B16, bool CAP, int PER> void go_verify(const VerifyArgs &a, hipStream_t s) {
     const unsigned rows = (unsigned)a.n_seqs * (a.max_drafts + 1), chunks = (unsigned)a.chunks, seqs = (unsigned)a.n_seqs;
-    hipLaunchKernelGGL((k_verify_stats<B16, PER>), dim3(rows * chunks), dim3(VF_THREADS), 0, s, a);
-    hipLaunchKernelGGL((k_verify_decide<B16, PER>), dim3(a.k > 0.0 ? seqs * chunks : seqs), dim3(VF_THREADS), 0, s, a);
-    if (a.k > 0.0) hipLaunchKernelGGL((k_verify_draw<B16, PER>), dim3(seqs), dim3(VF_THREADS), 0, s, a);
+    hipLaunchKernelGGL((k_verify_stats<B16, CAP, PER>), dim3(rows * chunks), dim3(VF_THREADS), 0, s, a);
+    hipLaunchKernelGGL((k_verify_decide<B16, CAP, PER>), dim3(a.k > 0.0 ? seqs * chunks : seqs), dim3(VF_THREADS), 0, s, a);
+    if (a.k > 0.0) hipLaunchKernelGGL((k_verify_draw<B16, CAP, PER>), dim3(seqs), dim3(VF_THREADS), 0, s, a);
+}
+
+template <bool B16> void go_verify(const VerifyArgs &a, int per, hipStream_t s) {
+    if (a.cap > 0.0) { if (per == 4) go_verify<B16, true, 4>(a, s); else go_verify<B16, true, 16>(a, s); }
+    else { if (per == 4) go_verify<B16, false, 4>(a, s); else go_verify<B16, false, 16>(a, s); }
 }
 
 }  // namespace
@@ -274,8 +279,7 @@ int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t wor
                        (int)d->n_seqs, (int)d->max_drafts, (int)d->vocab, c.n, greedy ? 0.0 : log2e / (double)d->temperature,
                        cap, cap > 0.0 ? 2.0 * log2e / cap : 0.0, st, (double *)(places + d->n_seqs), places, d->d_tokens, d->d_accepted};
     hipStream_t s = (hipStream_t)stream;
-    if (d->dtype == HIPDEC_ROWS_BF16) { if (c.per == 4) go_verify<true, 4>(a, s); else go_verify<true, 16>(a, s); }
-    else { if (c.per == 4) go_verify<false, 4>(a, s); else go_verify<false, 16>(a, s); }
+    if (d->dtype == HIPDEC_ROWS_BF16) go_verify<true>(a, c.per, s); else go_verify<false>(a, c.per, s);
     return launched(me);
 }
 
