@@ -16,7 +16,7 @@
 #define VF_THREADS 256
 #define VF_WAVES (VF_THREADS / WAVE)
 
-struct VfStat { double sum; float top; uint32_t arg; };      // of one chunk of one row: max logit, its first index, sum of weights
+struct VfStat { double sum; float top; uint32_t arg; };      // of one chunk of one row: max logit, the sum of weights (T > 0) or the maximum's first index (T = 0; else 0xffffffff)
 struct VfPlace { double inv; float top; int kept; };         // where a sequence's next token is drawn: 1 / the row's sum (0: nothing to draw), its maximum
 
 struct VerifyArgs {
@@ -40,15 +40,32 @@ __device__ __forceinline__ int vf_drafts(const VerifyArgs &a, int s) {
 template <bool B16> __device__ __forceinline__ float vf_logit(const VerifyArgs &a, long long row, int i) {
     const long long at = row * a.row_stride + i;
     const float x = B16 ? bf16_to_f32(((const uint16_t *)a.logits)[at]) : ((const float *)a.logits)[at];
-    return x == x ? x : -INFINITY;                           // a NaN is no possible token
+    return fminf(x == x ? x : -INFINITY, 3.4028235e38f);     // a NaN is no possible token; infinite ones share the whole
+}
+// PER logits of a thread: those of its chunk, VF_THREADS apart, or neighbours; -inf behind the vocabulary
+template <bool B16, int PER, bool NEAR> __device__ __forceinline__ void vf_logits(const VerifyArgs &a, long long row, int chunk, float *x) {
+    const int first = chunk * PER * VF_THREADS;
+    const bool inside = first + PER * VF_THREADS <= a.vocab;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = NEAR ? first + (int)threadIdx.x * PER + i : first + i * VF_THREADS + (int)threadIdx.x;
+        x[i] = inside || at < a.vocab ? vf_logit<B16>(a, row, at) : -INFINITY;
+    }
+}
+// the draft's probabilities of the same tokens
+template <int PER, bool NEAR> __device__ __forceinline__ void vf_guess(const VerifyArgs &a, long long draft, int chunk, float *q) {
+    const int first = chunk * PER * VF_THREADS, d = a.drafts[draft];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = NEAR ? first + (int)threadIdx.x * PER + i : first + i * VF_THREADS + (int)threadIdx.x;
+        q[i] = !a.probs ? d == at ? 1.0f : 0.0f : at < a.vocab ? a.probs[draft * a.prob_stride + at] : 0.0f;
+    }
 }
 
-// 2^y for y <= 1022: y = n + f with |f| <= 1/2, the series of 2^f = e^(f ln 2) up to its 11th power (the rest is below
-// 0.3466^12 / 12! = 7e-15 of it), scaled by 2^n in the exponent's bits.  n is read off the last bits of y + 1.5 * 2^52.
-// Below 2^-1020 the result stays there.  (These kernels are bound by this: with the library's exp, and conversions
-// and ldexp, which run at a quarter of the rate, the largest case takes 295 us, so XX.)
+// 2^y for -1021 <= y <= 1022: y = n + f with |f| <= 1/2, the series of 2^f = e^(f ln 2) up to its 11th power (the rest
+// is below 0.3466^12 / 12! = 7e-15 of it), scaled by 2^n in the exponent's bits.  n is read off the last bits of
+// y + 1.5 * 2^52.  The kernels' time on large calls is their instructions, most of them these 19 for each logit.
 __device__ __forceinline__ double vf_exp2(double y) {
-    y = fmax(y, -1020.0);
     const double whole = 6755399441055744.0, t = y + whole, f = y - (t - whole);
     double p = 4.4455382718708116e-10;                       // (ln 2)^k / k!, k = 11 .. 0
     p = fma(p, f, 7.054911620801123e-09);
@@ -68,18 +85,23 @@ __device__ __forceinline__ double vf_exp2(double y) {
 // the exponent behind it needs
 template <bool CAP> __device__ __forceinline__ double vf_capped(const VerifyArgs &a, float x) {
     if (!CAP) return (double)x;
-    const double d = vf_exp2(fmin((double)x * a.cap_k, 1000.0)) + 1.0;
+    const double d = vf_exp2(fmin(fmax((double)x * a.cap_k, -1000.0), 1000.0)) + 1.0;
     double r = __builtin_amdgcn_rcp(d);                      // 1 / d by Newton's method: each step squares the error
     r = fma(r, fma(-d, r, 1.0), r);
     r = fma(r, fma(-d, r, 1.0), r);
     return fma(-2.0 * a.cap, r, a.cap);
 }
-// exp((z - max z) / T); the maximum's own weight is 1 also where it is infinite, an impossible token's is 0.
-// ztop = vf_capped(top).  (Selections, not branches: the exponentials of a thread's logits run side by side.)
-template <bool CAP> __device__ __forceinline__ double vf_weight(const VerifyArgs &a, float x, float top, double ztop) {
-    const double w = vf_exp2((vf_capped<CAP>(a, x) - ztop) * a.k);
-    return x == -INFINITY ? 0.0 : x == top ? 1.0 : w;
+// exp((z - max z) / T) with ztop = the row's maximum z; impossible tokens, and what lies 2^1021 below the maximum, are 0.
+// EXACT_ZERO: whether the difference of 0 and 2^-1021 counts (it does where a token is picked, not in a row's sum).
+template <bool CAP, bool EXACT_ZERO> __device__ __forceinline__ double vf_weight(const VerifyArgs &a, float x, double ztop) {
+    const double y = fmax((vf_capped<CAP>(a, x) - ztop) * a.k, -1021.0);   // (a row of nothing else: -inf + inf, a NaN, counts as -1021)
+    const double w = vf_exp2(y);
+    if (CAP) return x == -INFINITY ? 0.0 : w;
+    return EXACT_ZERO ? y > -1021.0 ? w : 0.0 : w;
 }
+// max(p - q, 0), a NaN in q leaves 0.  (One fused operation wherever it is taken: a chunk whose sum is above 0 holds a
+// token that is.)
+__device__ __forceinline__ double vf_rest(double weight, double inv, float q) { return fmax(fma(weight, inv, -(double)q), 0.0); }
 __device__ __forceinline__ double vf_wave_sum(double v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
@@ -97,31 +119,36 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
     float x[PER];
     const bool unused = row - s * (a.max_drafts + 1) > vf_drafts(a, s);
     if (PER > 4 && unused) return;                           // (few logits are asked for without waiting for the draft's length)
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int at = (chunk * PER + i) * VF_THREADS + tid;
-        x[i] = at < a.vocab ? vf_logit<B16>(a, row, at) : -INFINITY;
-    }
+    vf_logits<B16, PER, false>(a, row, chunk, x);
     if (unused) return;
-    float top = -INFINITY; uint32_t arg = 0xffffffffu;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (x[i] > top) { top = x[i]; arg = (uint32_t)((chunk * PER + i) * VF_THREADS + tid); }
-    wave_argbest(top, arg);
-    if (lane == 0) { st[wave] = top; si[wave] = arg; }
-    __syncthreads();
-    top = st[0]; arg = si[0];
-#pragma unroll
-    for (int w = 1; w < VF_WAVES; ++w) if (better(st[w], si[w], top, arg)) { top = st[w]; arg = si[w]; }
+    float top = x[0];
+    uint32_t arg = 0xffffffffu;
     double sum = 0.0;
     if (a.k > 0.0) {
+#pragma unroll
+        for (int i = 1; i < PER; ++i) top = fmaxf(top, x[i]);
+        top = wave_max(top);
+        if (lane == 0) st[wave] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(st[0], st[1]), fmaxf(st[2], st[3]));
         const double ztop = vf_capped<CAP>(a, top);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) sum += vf_weight<CAP>(a, x[i], top, ztop);
+        for (int i = 0; i < PER; ++i) sum += vf_weight<CAP, false>(a, x[i], ztop);
         sum = vf_wave_sum(sum);
         if (lane == 0) ss[wave] = sum;
         __syncthreads();
-        sum = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+        sum = top == -INFINITY ? 0.0 : (ss[0] + ss[1]) + (ss[2] + ss[3]);
+    } else {
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (x[i] > top) { top = x[i]; arg = (uint32_t)((chunk * PER + i) * VF_THREADS + tid); }
+        wave_argbest(top, arg);
+        if (lane == 0) { st[wave] = top; si[wave] = arg; }
+        __syncthreads();
+        top = st[0]; arg = si[0];
+#pragma unroll
+        for (int w = 1; w < VF_WAVES; ++w) if (better(st[w], si[w], top, arg)) { top = st[w]; arg = si[w]; }
     }
     if (tid == 0) a.stats[(size_t)row * a.chunks + chunk] = VfStat{sum, top, arg};
 }
@@ -153,16 +180,18 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
         const double u = a.k > 0.0 && i < n ? (double)a.u[(size_t)s * (K + 1) + i] : 0.0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) if (better(mine[j].top, mine[j].arg, top, arg)) { top = mine[j].top; arg = mine[j].arg; }
-        wave_argbest(top, arg);
         double sum = 0.0, ztop = 0.0;
         if (a.k > 0.0) {
+            top = wave_max(top);
             ztop = vf_capped<CAP>(a, top);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (64 * j < a.chunks) sum += mine[j].sum * vf_weight<CAP>(a, mine[j].top, top, ztop);
+            for (int j = 0; j < 4; ++j) if (64 * j < a.chunks) sum += mine[j].sum * vf_weight<CAP, true>(a, mine[j].top, ztop);
             sum = vf_wave_sum(sum);
+        } else {
+            wave_argbest(top, arg);
         }
         const double inv = sum > 0.0 ? 1.0 / sum : 0.0;
-        const bool keep = real && (a.k > 0.0 ? u * q < vf_weight<CAP>(a, x, top, ztop) * inv : (uint32_t)d == arg);
+        const bool keep = real && (a.k > 0.0 ? u * q < vf_weight<CAP, true>(a, x, ztop) * inv : (uint32_t)d == arg);
         if (lane == 0) {
             s_inv[i] = inv; s_top[i] = top; s_arg[i] = arg;
             if (i < n && !keep) atomicMin(&s_kept, i);
@@ -183,16 +212,11 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
     const long long row = (long long)s * (K + 1) + kept, dr = (long long)s * K + kept;
     const double ztop = vf_capped<CAP>(a, top);
     float x[PER], q[PER];
-    const int d = a.drafts[dr];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int i = (part * PER + j) * VF_THREADS + tid;
-        x[j] = i < a.vocab ? vf_logit<B16>(a, row, i) : -INFINITY;
-        q[j] = i < a.vocab ? a.probs ? a.probs[dr * a.prob_stride + i] : d == i ? 1.0f : 0.0f : 0.0f;
-    }
+    vf_logits<B16, PER, false>(a, row, part, x);
+    vf_guess<PER, false>(a, dr, part, q);
     double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) sum += fmax(vf_weight<CAP>(a, x[j], top, ztop) * inv - (double)q[j], 0.0);   // (a NaN in q leaves 0)
+    for (int j = 0; j < PER; ++j) sum += vf_rest(vf_weight<CAP, true>(a, x[j], ztop), inv, q[j]);
     sum = vf_wave_sum(sum);
     if (lane == 0) ss[wave] = sum;
     __syncthreads();
@@ -240,7 +264,7 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
     const bool rest = some != 0;
     if (!rest) {
         const VfStat st = tid < a.chunks ? a.stats[(size_t)row * a.chunks + tid] : VfStat{0.0, -INFINITY, 0u};
-        mine = st.sum * vf_weight<CAP>(a, st.top, at.top, ztop) * at.inv;
+        mine = st.sum * vf_weight<CAP, true>(a, st.top, ztop) * at.inv;
     }
     double before, whole;
     const double run = vf_scan(mine, w1, before, whole), border = (double)u * whole;
@@ -254,19 +278,14 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
     if (tid == chunk) left = border - before;
     const int i0 = (chunk * VF_THREADS + tid) * PER;         // in index order
     float x[PER], q[PER];
-    const int d = rest ? a.drafts[dr] : -1;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int i = i0 + j;
-        x[j] = i < a.vocab ? vf_logit<B16>(a, row, i) : -INFINITY;
-        q[j] = i < a.vocab && rest ? a.probs ? a.probs[dr * a.prob_stride + i] : d == i ? 1.0f : 0.0f : 0.0f;
-    }
+    vf_logits<B16, PER, true>(a, row, chunk, x);
+    if (rest) vf_guess<PER, true>(a, dr, chunk, q);
     double w[PER];
     mine = 0.0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const double p = vf_weight<CAP>(a, x[j], at.top, ztop) * at.inv;
-        w[j] = rest ? fmax(p - (double)q[j], 0.0) : p;
+        const double t = vf_weight<CAP, true>(a, x[j], ztop);
+        w[j] = rest ? vf_rest(t, at.inv, q[j]) : t * at.inv;
         mine += w[j];
     }
     double r;

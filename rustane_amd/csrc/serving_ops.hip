@@ -89,11 +89,12 @@ template <bool RB, bool CB> void go_rope(const RopeArgs &a, bool wide, unsigned 
     else hipLaunchKernelGGL((k_rope_append<RB, CB, 1>), dim3(grid), dim3(ROPE_THREADS), 0, s, a);
 }
 
-// Logits of a row per workgroup: 1024 where that makes few workgroups (the draw of one sequence is latency), else 4096
-// (fewer reductions, and less of the statistics to read back).  At most 256 chunks: a thread each.
+// Logits of a row per workgroup: 1024 where that makes few workgroups (the draw is latency: 18.1 us for five rows of
+// 32768 against 24, 33.8 us for 256 rows against 37), else 4096 (fewer reductions, and less of the statistics to read
+// back: 108 us for 384 rows of 131071 against 155).  At most 256 chunks: a thread each.
 struct Chunks { int per, n; };
 Chunks chunks_of(uint64_t rows, uint32_t vocab) {
-    const int per = rows * vocab <= (uint64_t)16 * kCus * 1024 ? 4 : 16;
+    const int per = rows * vocab <= (uint64_t)64 * kCus * 1024 ? 4 : 16;
     return Chunks{per, (int)((vocab + per * VF_THREADS - 1) / (per * VF_THREADS))};
 }
 uint64_t verify_bytes(uint64_t n_seqs, uint32_t max_drafts, int chunks) {
