@@ -380,7 +380,7 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
  * s * max_drafts + i; NULL: certain of its token), draft i is kept while d_uniforms[s][i] * q(draft) < p(draft); where
  * it is not, the next token is drawn from max(p - q, 0) (from p if that is zero everywhere), behind the last kept
  * draft from p: the lowest index whose running sum exceeds d_uniforms[s][max_drafts] times the whole sum, both in 64
- * bits.  temperature 0: p is certain of the largest logit (the lowest index of equals) and q of the draft, no random
+ * bits (a number of 1 or more, or a NaN: the last token with any probability).  temperature 0: p is certain of the largest logit (the lowest index of equals) and q of the draft, no random
  * number is used (d_uniforms may be NULL).  d_tokens[s][max_drafts + 1]: the kept drafts, the next token, then
  * 0xffffffff; d_accepted[s]: how many drafts were kept.  A draft outside the vocabulary is not kept; NaN logits are
  * impossible tokens, and so are those of -inf; a row of nothing else gives the next token 0xffffffff.  softcap <= 0:

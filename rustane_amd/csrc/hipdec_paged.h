@@ -142,9 +142,14 @@ template <bool RB, bool CB, int NP> __global__ __launch_bounds__(ROPE_THREADS) v
 // operand of one instruction).  Probabilities never leave their registers, nothing is transposed, the running
 // maximum and sum of a head sit in the lanes that hold its output, and P and V enter as fp32: a bf16 cache costs no
 // precision beyond its own.  The fp32 instruction has room: 64 cached numbers per 32 clocks and SIMD are 32 bytes a
-// clock and CU of a bf16 cache, three times what HBM delivers.
+// clock and CU of a bf16 cache, three times what HBM delivers.  FEW: up to four heads per key head use the 4 x 4 form
+// (16 independent blocks: four heads, the values of four dim groups and one of four keys), 64 numbers in 8 clocks; the
+// columns of the score tile then repeat every four, and the four lane groups keep sums over keys of their own.
+// (eight requests of 12 single heads 19.9 -> 17.2 us.)
 //   K of a bf16 cache goes into the bf16 instruction as it is; fp32 queries are three bf16 numbers each (24 bits),
 //   bf16 queries are one.  K of an fp32 cache uses the fp32 instruction.
+// Measured (MI355X, listed sizes): 64 requests of 1 .. 8192 slots, 32 heads over 8, bf16 (1.09 GB): 212 us, 5.2 TB/s; one
+// request of 65536: 54.7 us, 4.9 TB/s; 64 x 4096 evenly 5.5 TB/s; a large copy reaches 4.7.
 struct PagedAttn {
     PagedView c;
     const void *q;
@@ -177,19 +182,24 @@ template <int HD, bool CB, int NT> struct PagedTile {
     uint32_t v[NT][4][VW];
 };
 
-#define ATT_WAVES 4
+// Registers: a key and its value of one tile take hd * 2 (4) bytes / 64 each, for 16 lanes; with 16 keys to a block and three
+// workgroups a CU the other waves cover a wave's waits better than blocks of 32 keys with two (64 ragged requests 212
+// against 220 us; a second register set with the next block's loads under way gains nothing: the same bytes in flight).
 constexpr int att_tiles(int hd, bool cb) { return hd * (cb ? 2 : 4) <= 128 ? 2 : 1; }
 constexpr int att_groups(int hd, bool cb) { return hd * (cb ? 2 : 4) <= 256 ? 3 : hd * (cb ? 2 : 4) <= 512 ? 2 : 1; }
-template <int HD, bool QB, bool CB, bool FEW> __global__ __launch_bounds__(64 * ATT_WAVES, att_groups(HD, CB)) void k_attn_paged(PagedAttn a) {
+template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? att_groups(HD, CB) : 1) void k_attn_paged(PagedAttn a) {
     constexpr int NT = att_tiles(HD, CB);                    // key tiles of a block
     constexpr int KEYS = 16 * NT;
     using Tile = PagedTile<HD, CB, NT>;
     constexpr int KQ = Tile::KQ, NE = Tile::NE, VW = Tile::VW;
     constexpr int PARTS = QB ? 1 : 3;
     constexpr int QN = CB ? KQ * PARTS : KQ;
-    __shared__ __align__(16) float sm_o[ATT_WAVES * 16][8 * 16 + 4];
-    __shared__ float sm_m[ATT_WAVES][16], sm_l[ATT_WAVES][16];
+    constexpr int CE = CB && WAVES == 4 ? 8 : 4;              // value elements joined at a time
+    __shared__ __align__(16) float sm_o[WAVES * 16][CE * 16 + 4];
+    __shared__ float sm_m[WAVES][16], sm_l[WAVES][16];
 
+    // (rows and heads vary fastest: consecutive workgroups go to the eight XCDs in turn, and with the splits in front
+    // the XCD that gets a row's last split would be idle wherever rows are shorter than max_len: 320 against 220 us)
     const unsigned per = gridDim.x / a.splits;               // rows x units
     const int split = blockIdx.x / per, rest = blockIdx.x % per;
     const int units = a.c.kv_heads * a.tiles, row = rest / units, unit = rest % units;
@@ -209,10 +219,10 @@ template <int HD, bool QB, bool CB, bool FEW> __global__ __launch_bounds__(64 * 
     };
     int pg[NT], nx[NT];
     entry(wave, pg);
-    entry(wave + ATT_WAVES, nx);
+    entry(wave + WAVES, nx);
     if (lo >= hi) {
         if (a.splits == 1)                                   // nothing to attend to: zeros
-            for (int i = threadIdx.x; i < gn * HD; i += 64 * ATT_WAVES) {
+            for (int i = threadIdx.x; i < gn * HD; i += 64 * WAVES) {
                 const long long at = (long long)row * a.out_stride + (long long)head0 * HD + i;
                 if (QB) ((uint16_t *)a.out)[at] = 0; else ((float *)a.out)[at] = 0.0f;
             }
@@ -317,13 +327,14 @@ template <int HD, bool QB, bool CB, bool FEW> __global__ __launch_bounds__(64 * 
         pages(b, pg);
         load_k(b, pg, x);
         load_v(b, pg, x);
-        pages(b + ATT_WAVES, nx);
+        pages(b + WAVES, nx);
     }
-    for (; b < blocks; b += ATT_WAVES) {
+    for (; b < blocks; b += WAVES) {
         pg_f4 s[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             s[t] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            pg_f4 other = s[t];                              // (fp32: two sums, half the chain and less rounding)
 #pragma unroll
             for (int j = 0; j < KQ; ++j) {
                 if (CB) {
@@ -335,16 +346,19 @@ template <int HD, bool QB, bool CB, bool FEW> __global__ __launch_bounds__(64 * 
                     const uint32_t kw[4] = {x.k[t][j].x, x.k[t][j].y, x.k[t][j].z, x.k[t][j].w};
                     const uint32_t qw[4] = {qr[j].x, qr[j].y, qr[j].z, qr[j].w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
+                    for (int e = 0; e < 4; e += 2) {
                         s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e]), __uint_as_float(qw[e]), s[t], 0, 0, 0);
+                        other = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e + 1]), __uint_as_float(qw[e + 1]), other, 0, 0, 0);
+                    }
                 }
             }
+            if (!CB) s[t] += other;
         }
-        const bool more = b + ATT_WAVES < blocks;
+        const bool more = b + WAVES < blocks;
         bool gaps = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) gaps |= __ballot(pg[t] < 0) != 0;
-        if (more) load_k(b + ATT_WAVES, nx, x);
+        if (more) load_k(b + WAVES, nx, x);
         if (gaps)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -393,27 +407,28 @@ template <int HD, bool QB, bool CB, bool FEW> __global__ __launch_bounds__(64 * 
                     else acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(f, p[t][r], acc[e], 0, 0, 0);
                 }
         if (more) {
-            load_v(b + ATT_WAVES, nx, x);
+            load_v(b + WAVES, nx, x);
 #pragma unroll
             for (int t = 0; t < NT; ++t) pg[t] = nx[t];
-            entry(b + 2 * ATT_WAVES, nx);
-            pages(b + 2 * ATT_WAVES, nx);
+            entry(b + 2 * WAVES, nx);
+            pages(b + 2 * WAVES, nx);
         }
     }
 
     // the waves' shares joined in LDS and summed in a fixed order, up to 8 elements of each lane (128 dims) at a time.
     // Result row m of element e is dim m * ce + e - e0 of that part; with few heads a wave's four lane groups hold
     // sums over keys of their own, which are shares like those of the waves.
-    constexpr int HEADS = FEW ? 4 : 16, SHARES = 16 * ATT_WAVES / HEADS;
+    constexpr int HEADS = FEW ? 4 : 16, SHARES = 16 * WAVES / HEADS;
     l += __shfl_xor(l, 16, WAVE);
     l += __shfl_xor(l, 32, WAVE);
     if (lane < HEADS) { sm_m[wave][lane] = m; sm_l[wave][lane] = l; }
     const int row0 = FEW ? 4 * ((lane >> 2) & 3) : 4 * grp;
     const int mine = FEW ? (4 * wave + grp) * HEADS + qcol : wave * HEADS + col;
-    float M = -INFINITY, L = 0.0f, wt[ATT_WAVES];
+    float M = -INFINITY, L = 0.0f, wt[WAVES];
 #pragma unroll
-    for (int e0 = 0; e0 < NE; e0 += CB && NE - e0 >= 8 ? 8 : 4) {
-        const int ce = CB && NE - e0 >= 8 ? 8 : 4;           // 16 * ce dims of every head: 4 a thread, in rounds
+    for (int e0 = 0; e0 < NE; e0 += NE - e0 >= CE ? CE : 4) {
+        const int ce = NE - e0 >= CE ? CE : 4;               // 16 * ce dims of every head: 4 a thread, in rounds
+        const bool halves = CB && ce == 4 && e0 < NE / 8 * 8;    // of a piece of 8 elements: 4 dims of every 8
         if (e0) __syncthreads();
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -423,15 +438,16 @@ template <int HD, bool QB, bool CB, bool FEW> __global__ __launch_bounds__(64 * 
                     make_float4(acc[e0 + e][r], acc[e0 + e + 1][r], acc[e0 + e + 2][r], acc[e0 + e + 3][r]);
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < (HEADS * 4 * ce + 64 * ATT_WAVES - 1) / (64 * ATT_WAVES); ++i) {
-            const int at = i * 64 * ATT_WAVES + (int)threadIdx.x, head = at / (4 * ce), d = at % (4 * ce) * 4;
+        for (int i = 0; i < (HEADS * 4 * ce + 64 * WAVES - 1) / (64 * WAVES); ++i) {
+            const int at = i * 64 * WAVES + (int)threadIdx.x, head = at / (4 * ce), d = at % (4 * ce) * 4;
+            const int dim = halves ? 16 * (e0 & ~7) + 2 * d + (e0 & 7) : 16 * e0 + d;
             if (head >= gn) continue;
             M = -INFINITY; L = 0.0f;
 #pragma unroll
-            for (int w = 0; w < ATT_WAVES; ++w) M = fmaxf(M, sm_m[w][head]);
+            for (int w = 0; w < WAVES; ++w) M = fmaxf(M, sm_m[w][head]);
             const float ms = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-            for (int w = 0; w < ATT_WAVES; ++w) { wt[w] = __builtin_amdgcn_exp2f(sm_m[w][head] - ms); L = fmaf(wt[w], sm_l[w][head], L); }
+            for (int w = 0; w < WAVES; ++w) { wt[w] = __builtin_amdgcn_exp2f(sm_m[w][head] - ms); L = fmaf(wt[w], sm_l[w][head], L); }
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int k = 0; k < SHARES; ++k) {
@@ -442,10 +458,10 @@ template <int HD, bool QB, bool CB, bool FEW> __global__ __launch_bounds__(64 * 
             if (a.splits == 1) {
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
                 float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-                pg_put_n<QB, 4>(a.out, (long long)row * a.out_stride + (long long)(head0 + head) * HD + 16 * e0 + d, y);
+                pg_put_n<QB, 4>(a.out, (long long)row * a.out_stride + (long long)(head0 + head) * HD + dim, y);
             } else {
                 const size_t slot = ((size_t)row * a.heads + head0 + head) * a.splits + split;
-                *(float4 *)(a.part_o + slot * HD + 16 * e0 + d) = o;
+                *(float4 *)(a.part_o + slot * HD + dim) = o;
                 if (e0 == 0 && d == 0) *(float2 *)(a.part_ml + 2 * slot) = make_float2(M, L);
             }
         }

@@ -267,8 +267,8 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
         mine = st.sum * vf_weight<CAP, true>(a, st.top, ztop) * at.inv;
     }
     double before, whole;
-    const double run = vf_scan(mine, w1, before, whole), border = (double)u * whole;
-    // (no chunk passes the border where the random number is 1 or the sums round down: the last one with any weight)
+    // (a random number of 1 or more, or none: no running sum passes the border, and the last possible token it is)
+    const double run = vf_scan(mine, w1, before, whole), border = u < 1.0f ? (double)u * whole : INFINITY;
     if (mine > 0.0) {
         atomicMax(&last_chunk, tid);
         if (run > border) atomicMin(&hit_chunk, tid);

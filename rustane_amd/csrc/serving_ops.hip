@@ -62,22 +62,37 @@ PagedView view(const hipdec_paged_cache &c) {
     return v;
 }
 
-// Keys per split of the cache's length: a multiple of what the workgroup's waves take at once.
+// How the cache's length is split: keys per split (whole steps of 128, what the four waves of a workgroup take twice
+// each) and splits; one split means one launch of eight-wave workgroups that write the result themselves.
+//   * One workgroup per row and key head where the length is at most 256 (a step per wave; 8.9 us against 10.9 with the
+//     second launch), and up to 1024 where there are enough of them for most CUs (256 workgroups: 400 keys 13.4 us
+//     against 15.7).  Longer, it would win 4 % where all rows are equally long (64 x 8 heads of 4096: 185 us against
+//     194), but the longest row alone sets the end where they are not (16 rows of up to 16384: 243 us against 121), and
+//     the lengths are known on the device only.
+//   * Else two workgroups a CU, with at most 1024 keys each: fewer leave CUs idle, more pay in the latency each starts
+//     with (one request of 65536: 54.7 us, with four 59), longer ones end unevenly.
 struct Split { int chunk, splits; };
 Split split_of(uint64_t n_rows, uint32_t kv_heads, uint32_t g, uint64_t max_len) {
     const uint64_t units = n_rows * kv_heads * ((g + 15) / 16), steps = (max_len + 127) / 128;
+    if (max_len <= 256 || (units >= 192 && max_len <= 1024)) return Split{(int)(steps ? steps : 1) * 128, 1};
     const uint64_t want = units ? (2 * kCus + units - 1) / units : 1;
     uint64_t per = (steps + want - 1) / want;
-    if (per < 1) per = 1;
     if (per > 8) per = 8;
-    if (steps <= per) return Split{(int)(steps ? steps : 1) * 128, 1};
     return Split{(int)per * 128, (int)((steps + per - 1) / per)};
 }
 
+template <int HD, bool QB, bool CB, bool FEW> void go_attention(const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
+    // (eight waves of the widest fp32 heads would not keep their registers)
+    constexpr int WIDE = HD * (CB ? 2 : 4) <= 512 ? 8 : 4;
+    if (a.splits == 1) {
+        hipLaunchKernelGGL((k_attn_paged<HD, QB, CB, FEW, WIDE>), dim3(grid), dim3(64 * WIDE), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((k_attn_paged<HD, QB, CB, FEW, 4>), dim3(grid), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_attn_paged_join<HD, QB>), dim3(joins), dim3(256), 0, s, a);
+    }
+}
 template <int HD, bool QB, bool CB> void go_attention(const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
-    if (a.g <= 4) hipLaunchKernelGGL((k_attn_paged<HD, QB, CB, true>), dim3(grid), dim3(64 * ATT_WAVES), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_paged<HD, QB, CB, false>), dim3(grid), dim3(64 * ATT_WAVES), 0, s, a);
-    if (joins) hipLaunchKernelGGL((k_attn_paged_join<HD, QB>), dim3(joins), dim3(256), 0, s, a);
+    if (a.g <= 4) go_attention<HD, QB, CB, true>(a, grid, joins, s); else go_attention<HD, QB, CB, false>(a, grid, joins, s);
 }
 template <int HD> void go_attention(bool qb, bool cb, const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
     if (qb) { if (cb) go_attention<HD, true, true>(a, grid, joins, s); else go_attention<HD, true, false>(a, grid, joins, s); }
@@ -231,7 +246,7 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
                 g, tiles, (int)(rows->max_len < slots ? rows->max_len : slots), p.chunk, p.splits,
                 rows->scale * 1.44269504088896340736f, po, po + rows->n_rows * rows->heads * p.splits * cache->hd};
     const bool qb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;
-    const unsigned nj = p.splits > 1 ? (unsigned)joins : 0;
+    const unsigned nj = (unsigned)joins;
     hipStream_t s = (hipStream_t)stream;
     switch (cache->hd) {
     case 64: go_attention<64>(qb, cb, a, (unsigned)grid, nj, s); break;

@@ -298,6 +298,10 @@ class _Drafts(C.Structure):
                 ("d_tokens", C.c_void_p), ("d_accepted", C.c_void_p)]
 
 
+def _first(*values):
+    return next(v for v in values if v is not None)
+
+
 def _op_chk(lib, rc):
     if rc != OK:
         raise HipDecodeError(rc, (lib.hipdec_last_error(None) or b"").decode())
@@ -319,8 +323,9 @@ def rope_append_paged(rope, cache, q, k, v, q_out, positions, n_rows, heads, dty
     one row (a fused projection); left out, rows are dense."""
     lib = load_library()
     wide, kv_wide = heads * cache.hd, cache.kv_heads * cache.hd
-    rows = _NewRows(q, k, v, q_out, dtype, heads, n_rows, q_stride or row_stride or wide, k_stride or row_stride or kv_wide,
-                    v_stride or row_stride or kv_wide, q_out_stride or wide, positions, slots, seqs)
+    rows = _NewRows(q, k, v, q_out, dtype, heads, n_rows, _first(q_stride, row_stride, wide),
+                    _first(k_stride, row_stride, kv_wide), _first(v_stride, row_stride, kv_wide), _first(q_out_stride, wide),
+                    positions, slots, seqs)
     _op_chk(lib, lib.hipdec_rope_append_paged(C.byref(rope), C.byref(cache), C.byref(rows), stream))
 
 
@@ -335,8 +340,9 @@ def attention_paged(cache, q, out, lens, n_rows, heads, max_len, dtype=RowDtype.
                     out_stride=None, workspace=None, workspace_bytes=0, stream=None):
     """hipdec_attention_paged; scale: 1 / sqrt(hd) if left out, strides in elements (dense rows if left out)."""
     lib = load_library()
-    rows = _AttentionRows(q, out, dtype, heads, n_rows, q_stride or heads * cache.hd, out_stride or heads * cache.hd, lens,
-                          seqs, max_len, cache.hd ** -0.5 if scale is None else scale)
+    rows = _AttentionRows(q, out, dtype, heads, n_rows, _first(q_stride, heads * cache.hd),
+                          _first(out_stride, heads * cache.hd), lens,
+                          seqs, max_len, max(cache.hd, 1) ** -0.5 if scale is None else scale)
     _op_chk(lib, lib.hipdec_attention_paged(C.byref(cache), C.byref(rows), workspace, workspace_bytes, stream))
 
 
@@ -352,8 +358,8 @@ def verify_drafts(logits, drafts, uniforms, tokens, accepted, n_seqs, max_drafts
                   workspace_bytes=0, stream=None):
     """hipdec_verify_drafts; strides in elements (dense rows if left out)."""
     lib = load_library()
-    d = _Drafts(logits, dtype, vocab, n_seqs, max_drafts, temperature, softcap, row_stride or vocab, prob_stride or vocab,
-                drafts, n_drafts, draft_probs, uniforms, tokens, accepted)
+    d = _Drafts(logits, dtype, vocab, n_seqs, max_drafts, temperature, softcap, _first(row_stride, vocab),
+                _first(prob_stride, vocab), drafts, n_drafts, draft_probs, uniforms, tokens, accepted)
     _op_chk(lib, lib.hipdec_verify_drafts(C.byref(d), workspace, workspace_bytes, stream))
 
 
