@@ -173,13 +173,23 @@ __device__ __forceinline__ int pg_len(const PagedAttn &a, int row, int &seq) {
     return 0;
 }
 
-// The keys and values of one block of NT x 16 slots, in registers.
+// The keys and values of one block of NT x 16 slots, in registers.  (Whole vectors per load: with the words of a load as
+// single variables this compiler lets go of some of them while they are still to be read.)
+typedef uint32_t pg_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t pg_u2 __attribute__((ext_vector_type(2)));
 template <int HD, bool CB, int NT> struct PagedTile {
     static constexpr int KQ = HD * (CB ? 2 : 4) / 64;        // 16-byte pieces of a key per lane (4 lanes a key)
     static constexpr int NE = HD / 16;                       // elements of a value per lane (16 lanes a value)
-    static constexpr int VW = CB ? NE / 2 : NE;              // ... in dwords
-    uint4 k[NT][KQ];
-    uint32_t v[NT][4][VW];
+    static constexpr int VQ = (CB ? NE / 2 : NE) / 4;        // ... in 16-byte pieces
+    static constexpr bool TAIL = CB && NE % 8;               // ... and one of 8 bytes
+    pg_u4 k[NT][KQ], v[NT][4][VQ ? VQ : 1];
+    pg_u2 tail[NT][4];
+    // element e of key r's value as fp32
+    __device__ __forceinline__ float value(int t, int r, int e) const {
+        const int w = CB ? e / 2 : e;
+        const uint32_t u = TAIL && w >= 4 * VQ ? tail[t][r][w % 4] : v[t][r][w / 4][w % 4];
+        return __uint_as_float(!CB ? u : e % 2 ? u & 0xffff0000u : u << 16);
+    }
 };
 
 // Registers: a key and its value of one tile take hd * 2 (4) bytes / 64 each, for 16 lanes; with 16 keys to a block and three
@@ -191,7 +201,7 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
     constexpr int NT = att_tiles(HD, CB);                    // key tiles of a block
     constexpr int KEYS = 16 * NT;
     using Tile = PagedTile<HD, CB, NT>;
-    constexpr int KQ = Tile::KQ, NE = Tile::NE, VW = Tile::VW;
+    constexpr int KQ = Tile::KQ, NE = Tile::NE, VQ = Tile::VQ;
     constexpr int PARTS = QB ? 1 : 3;
     constexpr int QN = CB ? KQ * PARTS : KQ;
     constexpr int CE = CB && WAVES == 4 ? 8 : 4;              // value elements joined at a time
@@ -285,7 +295,7 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
             const int s = lo + b * KEYS + 16 * t + col;
             const char *p = kb + pg_offset(a.c, max(pg[t], 0), s);
 #pragma unroll
-            for (int j = 0; j < KQ; ++j) x.k[t][j] = *(const uint4 *)(p + 64 * j);
+            for (int j = 0; j < KQ; ++j) x.k[t][j] = *(const pg_u4 *)(p + 64 * j);
         }
     };
     auto load_v = [&](int b, const int *pg, Tile &x) {
@@ -296,23 +306,9 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
                 const int s = lo + b * KEYS + 16 * t + 4 * grp + r;
                 const int page = __shfl(pg[t], 4 * grp + r, WAVE);
                 const char *p = vb + pg_offset(a.c, max(page, 0), s);
-                if (CB) {
 #pragma unroll
-                    for (int c = 0; c < NE / 8; ++c) {
-                        const uint4 w = *(const uint4 *)(p + 256 * c + 16 * col);
-                        x.v[t][r][4 * c] = w.x; x.v[t][r][4 * c + 1] = w.y; x.v[t][r][4 * c + 2] = w.z; x.v[t][r][4 * c + 3] = w.w;
-                    }
-                    if (NE % 8) {
-                        const uint2 w = *(const uint2 *)(p + 256 * (NE / 8) + 8 * col);
-                        x.v[t][r][VW - 2] = w.x; x.v[t][r][VW - 1] = w.y;
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < NE / 4; ++c) {
-                        const uint4 w = *(const uint4 *)(p + 256 * c + 16 * col);
-                        x.v[t][r][4 * c] = w.x; x.v[t][r][4 * c + 1] = w.y; x.v[t][r][4 * c + 2] = w.z; x.v[t][r][4 * c + 3] = w.w;
-                    }
-                }
+                for (int c = 0; c < VQ; ++c) x.v[t][r][c] = *(const pg_u4 *)(p + 256 * c + 16 * col);
+                if (Tile::TAIL) x.tail[t][r] = *(const pg_u2 *)(p + 256 * VQ + 8 * col);
             }
     };
 
@@ -321,7 +317,7 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
     for (int e = 0; e < NE; ++e) acc[e] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;                           // of head `col`: m the same in its four lanes, l each lane's own share
     const int blocks = (hi - lo + KEYS - 1) / KEYS;
-    Tile x;
+    Tile x = {};
     int b = wave;
     if (b < blocks) {
         pages(b, pg);
@@ -329,7 +325,7 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
         load_v(b, pg, x);
         pages(b + WAVES, nx);
     }
-    for (; b < blocks; b += WAVES) {
+    while (b < blocks) {
         pg_f4 s[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -343,7 +339,7 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
                         s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pg_bf8, x.k[t][j]),
                                                                        __builtin_bit_cast(pg_bf8, qr[p * KQ + j]), s[t], 0, 0, 0);
                 } else {
-                    const uint32_t kw[4] = {x.k[t][j].x, x.k[t][j].y, x.k[t][j].z, x.k[t][j].w};
+                    const pg_u4 kw = x.k[t][j];
                     const uint32_t qw[4] = {qr[j].x, qr[j].y, qr[j].z, qr[j].w};
 #pragma unroll
                     for (int e = 0; e < 4; e += 2) {
@@ -392,27 +388,28 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (__shfl(pg[t], 4 * grp + r, WAVE) < 0)
+                    if (__shfl(pg[t], 4 * grp + r, WAVE) < 0) {
 #pragma unroll
-                        for (int c = 0; c < VW; ++c) x.v[t][r][c] = 0;
+                        for (int c = 0; c < VQ; ++c) x.v[t][r][c] = pg_u4{0, 0, 0, 0};
+                        x.tail[t][r] = pg_u2{0, 0};
+                    }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int e = 0; e < NE; ++e) {
-                    const uint32_t w = x.v[t][r][CB ? e / 2 : e];
-                    const float f = __uint_as_float(!CB ? w : e % 2 ? w & 0xffff0000u : w << 16);
+                    const float f = x.value(t, r, e);
                     if (FEW) acc[e] = __builtin_amdgcn_mfma_f32_4x4x1f32(f, p[t][r], acc[e], 0, 0, 0);
                     else acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(f, p[t][r], acc[e], 0, 0, 0);
                 }
-        if (more) {
-            load_v(b + WAVES, nx, x);
+        if (!more) break;
+        b += WAVES;
+        load_v(b, nx, x);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) pg[t] = nx[t];
-            entry(b + 2 * WAVES, nx);
-            pages(b + 2 * WAVES, nx);
-        }
+        for (int t = 0; t < NT; ++t) pg[t] = nx[t];
+        entry(b + WAVES, nx);
+        pages(b + WAVES, nx);
     }
 
     // the waves' shares joined in LDS and summed in a fixed order, up to 8 elements of each lane (128 dims) at a time.

@@ -277,7 +277,7 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
     const int chunk = hit_chunk != 0x7fffffff ? hit_chunk : last_chunk;
     if (tid == chunk) left = border - before;
     const int i0 = (chunk * VF_THREADS + tid) * PER;         // in index order
-    float x[PER], q[PER];
+    float x[PER], q[PER] = {};
     vf_logits<B16, PER, true>(a, row, chunk, x);
     if (rest) vf_guess<PER, true>(a, dr, chunk, q);
     double w[PER];

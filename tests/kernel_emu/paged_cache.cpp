@@ -185,6 +185,8 @@ int main() {
     attention<128, true, true, false, 4>("k_attn_paged<128, bf16, bf16>, pages that do not exist", 16, 1, 4, false, {70, 33, 3}, {0, 1, 2}, 128, true);
     attention<64, false, false, true, 4>("k_attn_paged<64, fp32, fp32, few>, shared sequences, no such sequence", 4, 2, 8, true, {37, 38, 39, 20}, {0, 0, 0, -1}, 32, false);
     attention<64, false, true, false, 8>("k_attn_paged<64, fp32, bf16>, 18 heads, pages of one slot", 18, 1, 1, false, {130, 17}, {0, 1}, 256, true);
+    attention<64, false, true, true, 8>("k_attn_paged<64, fp32, bf16, few>, one split", 1, 4, 16, false, {1, 17, 250, 0, 129}, {0, 1, 2, 3, 4}, 256, false);
+    attention<64, false, true, true, 4>("k_attn_paged<64, fp32, bf16, few>, splits", 2, 2, 16, true, {1, 17, 300, 0, 129}, {0, 1, 2, 3, 4}, 128, false);
     attention<192, true, true, true, 4>("k_attn_paged<192, bf16, bf16, few>", 2, 1, 32, true, {150}, {0}, 128, true);
     attention<256, false, false, false, 4>("k_attn_paged<256, fp32, fp32>", 5, 1, 16, false, {90, 2}, {0, 1}, 64, false);
     std::printf("%d checks failed\n", failures);
