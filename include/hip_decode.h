@@ -194,6 +194,33 @@ int hipdec_decode_token_block_stats_from_ids_batch(hipdec_model *m, const uint32
 int hipdec_materialize_current_logits_block_batch(hipdec_model *m, size_t row, size_t block_idx, float softcap,
                                                   float *out_logits, size_t cap, size_t *out_valid);
 
+/* ---- requests of their own prompts stepped together, with drafted tokens ----
+ *
+ * The reference serves one request at a time (bin/serve.rs).  Here sequences of different prompts and lengths
+ * share one pool of cache pages and every step streams the weights once for all of them; each may bring drafted
+ * tokens (from a smaller model, or looked up in its own text), of which the step keeps what the model agrees
+ * with.  hipdec_requests_open, once per model, allocates the pool (n_pages pages of page_size positions, a power
+ * of two, per layer) and room for max_seqs sequences.  hipdec_requests_admit copies the model's positions
+ * [0, len) into the pages of sequence `seq`: set the length to 0, prefill the prompt, admit it.
+ * hipdec_requests_release gives its pages back.  A batch (hipdec_batch_begin) must not be open.  The products
+ * are those of the multi-row step, so its demands on the model's dimensions hold (HIPDEC_ERR_UNSUPPORTED). */
+int hipdec_requests_open(hipdec_model *m, uint32_t page_size, uint32_t n_pages, uint32_t max_seqs);
+int hipdec_requests_admit(hipdec_model *m, uint32_t seq);
+int hipdec_requests_release(hipdec_model *m, uint32_t seq);
+/* positions sequence `seq` holds, and the pool's free pages (either may be NULL) */
+int hipdec_requests_len(const hipdec_model *m, uint32_t seq, size_t *out_len, size_t *out_free_pages);
+/* One step of n_seqs sequences, each named once in seqs[]: sequence i is fed tokens[i] and then its
+ * n_drafts[i] <= max_drafts (NULL: max_drafts) drafts, drafts[i][max_drafts]; n_seqs * (max_drafts + 1) <= 32.
+ * The decision is hipdec_verify_drafts' with host arrays: draft_probs[n_seqs][max_drafts][vocab] (NULL: the drafts
+ * are certain), uniforms[n_seqs][max_drafts + 1] in [0, 1) (may be NULL with temperature 0).
+ * out_tokens[n_seqs][max_drafts + 1]: the kept drafts, the next token (to be fed in the next step), then 0xffffffff;
+ * out_accepted[n_seqs]: how many drafts were kept.  The sequence grows by its token and the kept drafts.
+ * out_logits (nullable): [n_seqs][max_drafts + 1][vocab] raw logits, rows behind a sequence's drafts meaningless.
+ * HIPDEC_ERR_FULL, with nothing changed, where a sequence would pass cfg.seq or the pool has too few free pages. */
+int hipdec_requests_step(hipdec_model *m, size_t n_seqs, const uint32_t *seqs, const uint32_t *tokens, uint32_t max_drafts,
+                         const uint32_t *n_drafts, const uint32_t *drafts, const float *draft_probs, const float *uniforms,
+                         float temperature, float softcap, uint32_t *out_tokens, uint32_t *out_accepted, float *out_logits);
+
 /* Greedy run without a host round trip per token (the loop of engine/src/inference.rs:576-585):
  * starting from `token`, performs n_steps argmax steps, each feeding its result to the next;
  * out_tokens[n_steps].  Equivalent to n_steps calls of hipdec_decode_token_argmax_from_id. */
@@ -284,8 +311,8 @@ int hipdec_sample_fullvocab_noalloc(const float *d_logits, size_t vocab, const f
  * NULL = its default stream) without waiting for them, nothing is allocated and nothing is kept between
  * calls, so a call can be recorded into a graph.  Workspaces are the caller's: one per call in flight (two
  * streams, or two graphs that may run at once, need one each).  Structs are read before the call returns.
- * Errors are reported through hipdec_last_error(NULL) on the calling thread; after an error nothing was
- * enqueued.  Numbers in device memory cannot be checked on the host: what each call makes of those that are
+ * Errors are reported through hipdec_last_error(NULL) on the calling thread; after a refusal
+ * (HIPDEC_ERR_ARG, _UNSUPPORTED) nothing was enqueued.  Numbers in device memory cannot be checked on the host: what each call makes of those that are
  * out of range is said with it, and none leads outside the buffers described. */
 
 typedef enum {               /* number format of rows and logits */

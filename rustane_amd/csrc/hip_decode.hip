@@ -7,9 +7,11 @@
 #include "hipdec_prefill.h"
 #include "hipdec_batch.h"
 #include "hipdec_rows.h"
+#include "hipdec_requests.h"
 #include "hipdec_sample.h"
 
 #include <math.h>
+#include <cmath>
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
@@ -86,6 +88,25 @@ struct BatchState {
     const void *rows_suf_seen = nullptr; // first suffix cache the table was written for
 };
 
+// State of the requests stepped together over a paged cache (hipdec_requests.h).
+constexpr int kRequestRows = 32;         // rows of a step: tokens and drafts of all its sequences
+struct RequestState {
+    bool open = false;
+    int page_shift = 0, max_pages = 0;   // pages a sequence of cfg.seq positions needs
+    uint32_t max_seqs = 0, n_pages = 0;
+    std::vector<void *> k, v;            // per layer [n_pages][page][kv_dim]
+    std::vector<int> table;              // [max_seqs][max_pages], -1: none; d_table holds the same
+    std::vector<int> free_pages;
+    std::vector<long long> lens;         // positions held by each sequence, -1: not admitted
+    int *d_table = nullptr, *d_rows = nullptr, *h_rows = nullptr;   // d_rows / h_rows: [5][kRequestRows] positions, slots, sequences, lengths, drafts
+    double *d_freq = nullptr;
+    float *qkv = nullptr, *att = nullptr, *logits = nullptr, *d_u = nullptr, *h_u = nullptr, *d_probs = nullptr;
+    uint32_t *d_tok = nullptr, *h_tok = nullptr;                    // tokens of a step, then accepted counts
+    void *ws_att = nullptr, *ws_ver = nullptr;
+    uint64_t ws_att_bytes = 0, ws_ver_bytes = 0;
+    int *d_n = nullptr;                  // draft counts, behind the rows
+};
+
 }  // namespace
 
 // run state of the on-device sampler as the host stages it (pinned)
@@ -138,6 +159,7 @@ struct hipdec_model {
     size_t xslab_cap = 0;
     PrefillWork pf;
     BatchState bt;
+    RequestState rq;
     SampleParams *d_ss = nullptr;                     // on-device sampler (hipdec_sample.h)
     uint64_t *d_rng = nullptr;                        // [32], one state per row
     SampleHost *h_samp = nullptr;                     // pinned
@@ -1231,6 +1253,129 @@ int batch_fetch(hipdec_model *m, const void *dev, void *host, size_t floats) {
     return HIPDEC_OK;
 }
 
+// ---- requests of their own prompts stepped together over a paged cache (hipdec_requests.h)
+// an operator's refusal or failure as this model's
+#define OPCHK(expr) do { const int rc_ = (expr); if (rc_ != HIPDEC_OK) return fail(m, rc_, g_create_error.c_str()); } while (0)
+
+hipdec_paged_cache request_cache(const hipdec_model *m, uint32_t layer) {
+    const RequestState &r = m->rq;
+    const hipdec_config &c = m->cfg;
+    const int64_t page = (int64_t)1 << r.page_shift;
+    return hipdec_paged_cache{r.k[layer], r.v[layer], m->opt.kv_dtype, (uint32_t)page, r.n_pages, c.kv_heads, c.hd, r.max_seqs,
+                              (uint32_t)r.max_pages, r.d_table, page * c.kv_dim, (int64_t)c.kv_dim, (int64_t)c.hd};
+}
+
+int requests_open(hipdec_model *m, uint32_t page_size, uint32_t n_pages, uint32_t max_seqs) {
+    const hipdec_config &c = m->cfg;
+    RequestState &r = m->rq;
+    HCHK(hipSetDevice(m->opt.device));
+    while ((1u << r.page_shift) < page_size) ++r.page_shift;
+    r.max_pages = (int)((c.seq + page_size - 1) >> r.page_shift);
+    r.n_pages = n_pages;
+    r.max_seqs = max_seqs;
+    int rc;
+    const size_t bytes = (size_t)n_pages * page_size * c.kv_dim * (m->kvbf16 ? 2 : 4), N = c.q_dim + 2 * c.kv_dim, R = kRequestRows;
+    r.k.resize(c.nlayers, nullptr);
+    r.v.resize(c.nlayers, nullptr);
+    for (uint32_t l = 0; l < c.nlayers; ++l) {
+        if ((rc = dalloc(m, &r.k[l], bytes))) return rc;
+        if ((rc = dalloc(m, &r.v[l], bytes))) return rc;
+    }
+    r.table.assign((size_t)max_seqs * r.max_pages, -1);
+    r.lens.assign(max_seqs, -1);
+    r.free_pages.resize(n_pages);
+    for (uint32_t i = 0; i < n_pages; ++i) r.free_pages[i] = (int)(n_pages - 1 - i);
+    for (uint64_t rows = 1; rows <= R; ++rows) {
+        uint64_t need = 0;
+        for (uint64_t len = 0; len < c.seq + 128; len += 128) {
+            OPCHK(hipdec_attention_paged_workspace(rows, c.heads, c.kv_heads, c.hd, len, &need));
+            r.ws_att_bytes = std::max(r.ws_att_bytes, need);
+        }
+        for (uint32_t k = 0; rows * (k + 1) <= R; ++k) {
+            OPCHK(hipdec_verify_drafts_workspace(rows, k, c.vocab, &need));
+            r.ws_ver_bytes = std::max(r.ws_ver_bytes, need);
+        }
+    }
+    if ((rc = dalloc(m, &r.d_table, r.table.size() * 4))) return rc;
+    if ((rc = dalloc(m, &r.d_rows, 5 * R * 4))) return rc;
+    if ((rc = dalloc(m, &r.d_n, R * 4))) return rc;
+    if ((rc = dalloc(m, &r.d_freq, c.hd / 2 * sizeof(double)))) return rc;
+    if ((rc = dalloc(m, &r.qkv, R * N * 4))) return rc;
+    if ((rc = dalloc(m, &r.att, R * c.q_dim * 4))) return rc;
+    if ((rc = dalloc(m, &r.logits, R * c.vocab * 4))) return rc;
+    if ((rc = dalloc(m, &r.d_u, R * 4))) return rc;
+    if ((rc = dalloc(m, &r.d_tok, 2 * R * 4))) return rc;
+    if ((rc = dalloc(m, &r.ws_att, r.ws_att_bytes + 16))) return rc;
+    if ((rc = dalloc(m, &r.ws_ver, r.ws_ver_bytes + 16))) return rc;
+    HCHK(hipHostMalloc((void **)&r.h_rows, 6 * R * 4));
+    HCHK(hipHostMalloc((void **)&r.h_u, R * 4));
+    HCHK(hipHostMalloc((void **)&r.h_tok, 2 * R * 4));
+    // the angles of the model's own table (theta = pos / 10000^(2i / hd) in fp32, lib.rs:1401) as frequencies
+    std::vector<double> freq(c.hd / 2);
+    for (size_t i = 0; i < freq.size(); ++i) freq[i] = 1.0 / (double)powf(10000.0f, 2.0f * (float)i / (float)c.hd);
+    HCHK(hipMemcpy(r.d_freq, freq.data(), freq.size() * sizeof(double), hipMemcpyHostToDevice));
+    HCHK(hipMemcpy(r.d_table, r.table.data(), r.table.size() * 4, hipMemcpyHostToDevice));
+    r.open = true;
+    return HIPDEC_OK;
+}
+
+// gives sequence q the pages of positions [0, len); the caller has checked that there are enough
+void request_pages(hipdec_model *m, uint32_t q, size_t len) {
+    RequestState &r = m->rq;
+    int *row = &r.table[(size_t)q * r.max_pages];
+    for (size_t p = 0; p << r.page_shift < len; ++p)
+        if (row[p] < 0) { row[p] = r.free_pages.back(); r.free_pages.pop_back(); }
+}
+size_t request_pages_missing(const hipdec_model *m, uint32_t q, size_t len) {
+    const RequestState &r = m->rq;
+    const int *row = &r.table[(size_t)q * r.max_pages];
+    size_t n = 0;
+    for (size_t p = 0; p << r.page_shift < len; ++p) n += row[p] < 0;
+    return n;
+}
+int request_table_up(hipdec_model *m, uint32_t q) {
+    RequestState &r = m->rq;
+    const size_t at = (size_t)q * r.max_pages;
+    HCHK(hipMemcpyAsync(r.d_table + at, &r.table[at], (size_t)r.max_pages * 4, hipMemcpyHostToDevice, m->stream));
+    return HIPDEC_OK;
+}
+
+// the layers and the head for R rows whose ids, positions, slots, sequences and lengths are on the device
+int requests_forward(hipdec_model *m, int R, size_t max_len) {
+    const hipdec_config &c = m->cfg;
+    RequestState &r = m->rq;
+    PrefillWork &w = m->pf;
+    const int D = c.dim, Q = c.q_dim, KV = c.kv_dim, H = c.hidden, V = c.vocab, N = Q + 2 * KV;
+    const int nch = (D + PF_CHUNK - 1) / PF_CHUNK;
+    const hipdec_rope rope{r.d_freq, c.hd, 1, 1.0f};
+    pf_launch_embed(m, R);
+    for (uint32_t l = 0; l < c.nlayers; ++l) {
+        const DevLayer &L = m->layers[l];
+        const hipdec_paged_cache cache = request_cache(m, l);
+        int sp = pf_gemm(m, m->wt, w.xn_hi, w.xn_lo, L.wqkv, L.s_qkv, R, N, D);
+        hipLaunchKernelGGL(k_rq_qkv_rows, dim3((unsigned)((N / 2 + 255) / 256), (unsigned)R), dim3(256), 0, m->stream, w.P, sp, (size_t)R * N,
+                           m->wt == WT_FP8 ? (const float *)L.s_qkv : nullptr, r.qkv, w.ssq, nch, D, N);
+        const hipdec_new_rows rows{r.qkv, r.qkv + Q, r.qkv + Q + KV, w.q, HIPDEC_ROWS_F32, c.heads, (uint64_t)R, N, N, N, Q,
+                                   r.d_rows, r.d_rows + kRequestRows, r.d_rows + 2 * kRequestRows};
+        OPCHK(hipdec_rope_append_paged(&rope, &cache, &rows, m->stream));
+        const hipdec_attention_rows att{w.q, r.att, HIPDEC_ROWS_F32, c.heads, (uint64_t)R, Q, Q, r.d_rows + 3 * kRequestRows,
+                                        r.d_rows + 2 * kRequestRows, max_len, 1.0f / sqrtf((float)c.hd)};
+        OPCHK(hipdec_attention_paged(&cache, &att, r.ws_att, r.ws_att_bytes, m->stream));
+        hipLaunchKernelGGL(k_rq_pair, dim3((unsigned)((R * Q + 255) / 256)), dim3(256), 0, m->stream, r.att, w.att_hi, w.att_lo, R * Q);
+        sp = pf_gemm(m, m->wt, w.att_hi, w.att_lo, L.wo, L.s_wo, R, D, Q);
+        pf_launch_resid(m, R, sp, L.s_wo, w.x, w.x2, L.g2);
+        sp = pf_gemm(m, m->wt, w.xn_hi, w.xn_lo, L.w13, L.s_w13, R, 2 * H, D);
+        pf_launch_gate(m, R, sp, L.s_w13);
+        sp = pf_gemm(m, m->wt, w.gate_hi, w.gate_lo, L.w2, L.s_w2, R, D, H);
+        pf_launch_resid(m, R, sp, L.s_w2, w.x2, w.x, l + 1 < c.nlayers ? m->layers[l + 1].g1 : m->gfinal);
+    }
+    const int sp = pf_gemm(m, m->embed_wt, w.xn_hi, w.xn_lo, m->embed, nullptr, R, V, D);
+    const size_t n = (size_t)R * V;
+    hipLaunchKernelGGL(k_bd_sum_planes, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, m->stream, w.P, sp, n, r.logits, n, w.ssq, nch, D, V);
+    HCHK(hipGetLastError());
+    return HIPDEC_OK;
+}
+
 // ---- sampled runs that stay on the device (hipdec_sample.h)
 float sample_inv_temperature(float temperature) {              // engine/src/decode.rs:174
     const float tiny = 1.17549435e-38f;                        // f32::MIN_POSITIVE
@@ -1407,6 +1552,9 @@ void hipdec_destroy(hipdec_model *m) {
     if (m->bt.h_bp) (void)hipHostFree(m->bt.h_bp);
     if (m->bt.h_stage) (void)hipHostFree(m->bt.h_stage);
     if (m->bt.h_ring) (void)hipHostFree(m->bt.h_ring);
+    if (m->rq.h_rows) (void)hipHostFree(m->rq.h_rows);
+    if (m->rq.h_u) (void)hipHostFree(m->rq.h_u);
+    if (m->rq.h_tok) (void)hipHostFree(m->rq.h_tok);
     if (m->h_samp) (void)hipHostFree(m->h_samp);
     if (m->h_abort) (void)hipHostFree(m->h_abort);
     if (m->ev0) (void)hipEventDestroy(m->ev0);
@@ -2193,6 +2341,151 @@ int hipdec_materialize_current_logits_block_batch(hipdec_model *m, size_t row, s
     int rc = batch_fetch(m, b.d_out, out_logits, valid);
     if (rc) return rc;
     if (out_valid) *out_valid = valid;
+    return HIPDEC_OK;
+}
+
+int hipdec_requests_open(hipdec_model *m, uint32_t page_size, uint32_t n_pages, uint32_t max_seqs) {
+    if (!m) return HIPDEC_ERR_ARG;
+    if (m->rq.open) return fail(m, HIPDEC_ERR_ARG, "the model's pages are open already");
+    if (!page_size || (page_size & (page_size - 1)) || page_size > 65536) return fail(m, HIPDEC_ERR_ARG, "page_size must be a power of two up to 65536");
+    if (!n_pages || n_pages > 0x7fffffffu || !max_seqs || max_seqs > 65536) return fail(m, HIPDEC_ERR_ARG, "n_pages or max_seqs out of range");
+    if (!prefill_batched_ok(m, kPrefillMinRows) || m->cfg.vocab > 262144)
+        return fail(m, HIPDEC_ERR_UNSUPPORTED, "requests stepped together need dimensions that are multiples of 32 (128 with 4-bit weights), a head dimension of 64 or 128 and a vocabulary up to 262144");
+    const size_t had = m->allocs.size();
+    int rc;
+    try { rc = requests_open(m, page_size, n_pages, max_seqs); } catch (...) { rc = fail(m, HIPDEC_ERR_HIP, "out of host memory"); }
+    if (rc == HIPDEC_OK) return rc;
+    // too large a pool: everything back, so that a smaller one can be opened
+    RequestState &r = m->rq;
+    for (; m->allocs.size() > had; m->allocs.pop_back()) (void)hipFree(m->allocs.back());
+    if (r.h_rows) (void)hipHostFree(r.h_rows);
+    if (r.h_u) (void)hipHostFree(r.h_u);
+    if (r.h_tok) (void)hipHostFree(r.h_tok);
+    r = RequestState{};
+    (void)hipGetLastError();                                  // (the failed allocation's: it is reported, and must not be again)
+    return rc;
+}
+
+int hipdec_requests_admit(hipdec_model *m, uint32_t seq) {
+    if (!m) return HIPDEC_ERR_ARG;
+    RequestState &r = m->rq;
+    if (!r.open) return fail(m, HIPDEC_ERR_ARG, "no pages are open (hipdec_requests_open)");
+    if (m->bt.rows) return fail(m, HIPDEC_ERR_ARG, "a batch is open");
+    if (seq >= r.max_seqs || r.lens[seq] >= 0) return fail(m, HIPDEC_ERR_ARG, "sequence out of range or admitted already");
+    if (request_pages_missing(m, seq, m->len) > r.free_pages.size()) return fail(m, HIPDEC_ERR_FULL, "not enough free pages");
+    HCHK(hipSetDevice(m->opt.device));
+    HCHK(hipStreamSynchronize(m->stream));
+    request_pages(m, seq, m->len);
+    const int rc = request_table_up(m, seq);
+    if (rc) return rc;
+    const int pieces = (int)(m->cfg.kv_dim * (m->kvbf16 ? 2 : 4) / 16);
+    if (m->len)
+        for (uint32_t l = 0; l < m->cfg.nlayers; ++l) {
+            const DevLayer &L = m->layers[l];
+            for (int which = 0; which < 2; ++which)
+                hipLaunchKernelGGL(k_rq_admit, dim3((unsigned)m->len), dim3(256), 0, m->stream, (const uint4 *)(which ? L.vc : L.kc),
+                                   (uint4 *)(which ? r.v[l] : r.k[l]), r.d_table + (size_t)seq * r.max_pages, r.page_shift, pieces, (int)m->len);
+        }
+    HCHK(hipGetLastError());
+    HCHK(hipStreamSynchronize(m->stream));
+    r.lens[seq] = (long long)m->len;
+    return HIPDEC_OK;
+}
+
+int hipdec_requests_release(hipdec_model *m, uint32_t seq) {
+    if (!m) return HIPDEC_ERR_ARG;
+    RequestState &r = m->rq;
+    if (!r.open || seq >= r.max_seqs || r.lens[seq] < 0) return fail(m, HIPDEC_ERR_ARG, "no such sequence");
+    int *row = &r.table[(size_t)seq * r.max_pages];
+    for (int p = 0; p < r.max_pages; ++p)
+        if (row[p] >= 0) { r.free_pages.push_back(row[p]); row[p] = -1; }
+    r.lens[seq] = -1;
+    return HIPDEC_OK;
+}
+
+int hipdec_requests_len(const hipdec_model *m, uint32_t seq, size_t *out_len, size_t *out_free_pages) {
+    if (!m || !m->rq.open || seq >= m->rq.max_seqs || m->rq.lens[seq] < 0) return HIPDEC_ERR_ARG;
+    if (out_len) *out_len = (size_t)m->rq.lens[seq];
+    if (out_free_pages) *out_free_pages = m->rq.free_pages.size();
+    return HIPDEC_OK;
+}
+
+int hipdec_requests_step(hipdec_model *m, size_t n_seqs, const uint32_t *seqs, const uint32_t *tokens, uint32_t max_drafts,
+                         const uint32_t *n_drafts, const uint32_t *drafts, const float *draft_probs, const float *uniforms,
+                         float temperature, float softcap, uint32_t *out_tokens, uint32_t *out_accepted, float *out_logits) {
+    if (!m) return HIPDEC_ERR_ARG;
+    const hipdec_config &c = m->cfg;
+    RequestState &r = m->rq;
+    if (!r.open) return fail(m, HIPDEC_ERR_ARG, "no pages are open (hipdec_requests_open)");
+    if (m->bt.rows) return fail(m, HIPDEC_ERR_ARG, "a batch is open");
+    if (!seqs || !tokens || !out_tokens || !out_accepted || (max_drafts && !drafts)) return fail(m, HIPDEC_ERR_ARG, "null buffer");
+    if (!(temperature >= 0.0f) || !std::isfinite(temperature) || !(softcap <= 3.4e38f)) return fail(m, HIPDEC_ERR_ARG, "temperature must not be negative, softcap must be finite");
+    if (temperature > 0.0f && !uniforms) return fail(m, HIPDEC_ERR_ARG, "random numbers are missing");
+    const size_t K = max_drafts, S = K + 1;
+    if (n_seqs == 0 || n_seqs > (size_t)kRequestRows || S > (size_t)kRequestRows || n_seqs * S > (size_t)kRequestRows || n_seqs * S > c.seq)
+        return fail(m, HIPDEC_ERR_ARG, "n_seqs * (max_drafts + 1) must be in 1..32");
+    size_t missing = 0, max_len = 0;
+    for (size_t i = 0; i < n_seqs; ++i) {
+        if (seqs[i] >= r.max_seqs || r.lens[seqs[i]] < 0) return fail(m, HIPDEC_ERR_ARG, "no such sequence");
+        for (size_t j = 0; j < i; ++j) if (seqs[j] == seqs[i]) return fail(m, HIPDEC_ERR_ARG, "a sequence is named twice");
+        const size_t nd = n_drafts ? n_drafts[i] : K;
+        if (nd > K) return fail(m, HIPDEC_ERR_ARG, "more drafts than max_drafts");
+        if (tokens[i] >= c.vocab) return fail(m, HIPDEC_ERR_ARG, "token id must fit vocab");
+        for (size_t j = 0; j < nd; ++j) if (drafts[i * K + j] >= c.vocab) return fail(m, HIPDEC_ERR_ARG, "token id must fit vocab");
+        const size_t len = (size_t)r.lens[seqs[i]] + 1 + nd;
+        if (len > c.seq) return fail(m, HIPDEC_ERR_FULL, "decode only supports lengths within cfg.seq");
+        missing += request_pages_missing(m, seqs[i], len);
+        max_len = std::max(max_len, len);
+    }
+    if (missing > r.free_pages.size()) return fail(m, HIPDEC_ERR_FULL, "not enough free pages");
+
+    const int R = (int)(n_seqs * S);
+    HCHK(hipSetDevice(m->opt.device));
+    int rc = pf_ensure(m, R, true);
+    if (rc) return rc;
+    if (draft_probs && K && temperature > 0.0f && !r.d_probs && (rc = dalloc(m, &r.d_probs, (size_t)kRequestRows * c.vocab * 4))) return rc;
+    PrefillWork &w = m->pf;
+    HCHK(hipStreamSynchronize(m->stream));                      // pinned staging is free again
+    int *pos = r.h_rows, *slot = pos + kRequestRows, *sq = slot + kRequestRows, *ln = sq + kRequestRows, *dr = ln + kRequestRows, *nn = dr + kRequestRows;
+    for (size_t i = 0; i < n_seqs; ++i) {
+        const size_t nd = n_drafts ? n_drafts[i] : K, len = (size_t)r.lens[seqs[i]];
+        request_pages(m, seqs[i], len + 1 + nd);
+        if ((rc = request_table_up(m, seqs[i]))) return rc;
+        nn[i] = (int)nd;
+        for (size_t j = 0; j < S; ++j) {
+            const size_t row = i * S + j;
+            const bool real = j <= nd;                          // a row behind the sequence's drafts: written nowhere, sees nothing
+            w.h_ids[row] = !real ? 0 : j == 0 ? tokens[i] : drafts[i * K + j - 1];
+            pos[row] = real ? (int)(len + j) : 0;
+            slot[row] = real ? (int)(len + j) : -1;
+            sq[row] = (int)seqs[i];
+            ln[row] = real ? (int)(len + j + 1) : 0;
+            if (j < K) dr[i * K + j] = j < nd ? (int)drafts[i * K + j] : -1;
+            if (temperature > 0.0f) r.h_u[row] = uniforms[row];
+        }
+    }
+    HCHK(hipMemcpyAsync(w.ids, w.h_ids, (size_t)R * 4, hipMemcpyHostToDevice, m->stream));
+    HCHK(hipMemcpyAsync(r.d_rows, r.h_rows, 5 * kRequestRows * 4, hipMemcpyHostToDevice, m->stream));
+    HCHK(hipMemcpyAsync(r.d_n, nn, n_seqs * 4, hipMemcpyHostToDevice, m->stream));
+    if (temperature > 0.0f) HCHK(hipMemcpyAsync(r.d_u, r.h_u, (size_t)R * 4, hipMemcpyHostToDevice, m->stream));
+    const bool probs = draft_probs && K && temperature > 0.0f;
+    if (probs) HCHK(hipMemcpyAsync(r.d_probs, draft_probs, n_seqs * K * c.vocab * 4, hipMemcpyHostToDevice, m->stream));
+    HCHK(hipEventRecord(m->ev0, m->stream));
+    if ((rc = requests_forward(m, R, max_len))) return rc;
+    const hipdec_drafts v{r.logits, HIPDEC_ROWS_F32, c.vocab, n_seqs, max_drafts, temperature, softcap, (int64_t)c.vocab, (int64_t)c.vocab,
+                          r.d_rows + 4 * kRequestRows, r.d_n, probs ? r.d_probs : nullptr, r.d_u, r.d_tok, (int32_t *)r.d_tok + kRequestRows};
+    OPCHK(hipdec_verify_drafts(&v, r.ws_ver, r.ws_ver_bytes, m->stream));
+    HCHK(hipEventRecord(m->ev1, m->stream));
+    HCHK(hipMemcpyAsync(r.h_tok, r.d_tok, 2 * kRequestRows * 4, hipMemcpyDeviceToHost, m->stream));
+    if (out_logits) HCHK(hipMemcpyAsync(out_logits, r.logits, (size_t)R * c.vocab * 4, hipMemcpyDeviceToHost, m->stream));
+    HCHK(hipStreamSynchronize(m->stream));
+    HCHK(hipEventElapsedTime(&m->last_ms, m->ev0, m->ev1));
+    m->step_timed = false;
+    memcpy(out_tokens, r.h_tok, (size_t)R * 4);
+    for (size_t i = 0; i < n_seqs; ++i) {
+        out_accepted[i] = r.h_tok[kRequestRows + i];
+        r.lens[seqs[i]] += 1 + (long long)out_accepted[i];
+    }
     return HIPDEC_OK;
 }
 

@@ -17,10 +17,19 @@ constexpr uint64_t kMaxRows = 1u << 24, kMaxLen = 1u << 30;
 constexpr int kCus = 256;                                    // compute units of the one device this is built for
 
 int refuse(const char *entry, const char *what) { return hipdec_op_error(HIPDEC_ERR_ARG, entry, what); }
-int launched(const char *entry) {
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? HIPDEC_OK : hipdec_op_error(HIPDEC_ERR_HIP, entry, hipGetErrorString(e));
+int launched(const char *entry, hipError_t e) {
+    if (e == hipSuccess) return HIPDEC_OK;
+    (void)hipGetLastError();
+    return hipdec_op_error(HIPDEC_ERR_HIP, entry, hipGetErrorString(e));
 }
+// A launch with its own error, not whatever an earlier call of the program has left behind.
+template <typename A> hipError_t start(void (*kernel)(A), uint64_t grid, int threads, hipStream_t s, const A &a) {
+    void *args[] = {(void *)&a};
+    return hipLaunchKernel((const void *)kernel, dim3((unsigned)grid), dim3((unsigned)threads), args, 0, s);
+}
+
+// (a grid's threads are counted in 32 bits)
+bool grid_fits(uint64_t groups, uint64_t threads) { return groups <= 0x7fffffffu && groups * threads <= 0xffffffffu; }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -81,27 +90,23 @@ Split split_of(uint64_t n_rows, uint32_t kv_heads, uint32_t g, uint64_t max_len)
     return Split{(int)per * 128, (int)((steps + per - 1) / per)};
 }
 
-template <int HD, bool QB, bool CB, bool FEW> void go_attention(const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
+template <int HD, bool QB, bool CB, bool FEW> hipError_t go_attention(const PagedAttn &a, uint64_t grid, uint64_t joins, hipStream_t s) {
     // (eight waves of the widest fp32 heads would not keep their registers)
     constexpr int WIDE = HD * (CB ? 2 : 4) <= 512 ? 8 : 4;
-    if (a.splits == 1) {
-        hipLaunchKernelGGL((k_attn_paged<HD, QB, CB, FEW, WIDE>), dim3(grid), dim3(64 * WIDE), 0, s, a);
-    } else {
-        hipLaunchKernelGGL((k_attn_paged<HD, QB, CB, FEW, 4>), dim3(grid), dim3(256), 0, s, a);
-        hipLaunchKernelGGL((k_attn_paged_join<HD, QB>), dim3(joins), dim3(256), 0, s, a);
-    }
+    if (a.splits == 1) return start(k_attn_paged<HD, QB, CB, FEW, WIDE>, grid, 64 * WIDE, s, a);
+    const hipError_t e = start(k_attn_paged<HD, QB, CB, FEW, 4>, grid, 256, s, a);
+    return e != hipSuccess ? e : start(k_attn_paged_join<HD, QB>, joins, 256, s, a);
 }
-template <int HD, bool QB, bool CB> void go_attention(const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
-    if (a.g <= 4) go_attention<HD, QB, CB, true>(a, grid, joins, s); else go_attention<HD, QB, CB, false>(a, grid, joins, s);
+template <int HD, bool QB, bool CB> hipError_t go_attention(const PagedAttn &a, uint64_t grid, uint64_t joins, hipStream_t s) {
+    return a.g <= 4 ? go_attention<HD, QB, CB, true>(a, grid, joins, s) : go_attention<HD, QB, CB, false>(a, grid, joins, s);
 }
-template <int HD> void go_attention(bool qb, bool cb, const PagedAttn &a, unsigned grid, unsigned joins, hipStream_t s) {
-    if (qb) { if (cb) go_attention<HD, true, true>(a, grid, joins, s); else go_attention<HD, true, false>(a, grid, joins, s); }
-    else { if (cb) go_attention<HD, false, true>(a, grid, joins, s); else go_attention<HD, false, false>(a, grid, joins, s); }
+template <int HD> hipError_t go_attention(bool qb, bool cb, const PagedAttn &a, uint64_t grid, uint64_t joins, hipStream_t s) {
+    if (qb) return cb ? go_attention<HD, true, true>(a, grid, joins, s) : go_attention<HD, true, false>(a, grid, joins, s);
+    return cb ? go_attention<HD, false, true>(a, grid, joins, s) : go_attention<HD, false, false>(a, grid, joins, s);
 }
 
-template <bool RB, bool CB> void go_rope(const RopeArgs &a, bool wide, unsigned grid, hipStream_t s) {
-    if (wide) hipLaunchKernelGGL((k_rope_append<RB, CB, 4>), dim3(grid), dim3(ROPE_THREADS), 0, s, a);
-    else hipLaunchKernelGGL((k_rope_append<RB, CB, 1>), dim3(grid), dim3(ROPE_THREADS), 0, s, a);
+template <bool RB, bool CB> hipError_t go_rope(const RopeArgs &a, bool wide, uint64_t grid, hipStream_t s) {
+    return wide ? start(k_rope_append<RB, CB, 4>, grid, ROPE_THREADS, s, a) : start(k_rope_append<RB, CB, 1>, grid, ROPE_THREADS, s, a);
 }
 
 // Logits of a row per workgroup: 1024 where that makes few workgroups (the draw is latency: 18.1 us for five rows of
@@ -116,16 +121,16 @@ uint64_t verify_bytes(uint64_t n_seqs, uint32_t max_drafts, int chunks) {
     return n_seqs * ((max_drafts + 1) * chunks * sizeof(VfStat) + chunks * sizeof(double) + sizeof(VfPlace));
 }
 
-template <bool B16, bool CAP, int PER> void go_verify(const VerifyArgs &a, hipStream_t s) {
-    const unsigned rows = (unsigned)a.n_seqs * (a.max_drafts + 1), chunks = (unsigned)a.chunks, seqs = (unsigned)a.n_seqs;
-    hipLaunchKernelGGL((k_verify_stats<B16, CAP, PER>), dim3(rows * chunks), dim3(VF_THREADS), 0, s, a);
-    hipLaunchKernelGGL((k_verify_decide<B16, CAP, PER>), dim3(a.k > 0.0 ? seqs * chunks : seqs), dim3(VF_THREADS), 0, s, a);
-    if (a.k > 0.0) hipLaunchKernelGGL((k_verify_draw<B16, CAP, PER>), dim3(seqs), dim3(VF_THREADS), 0, s, a);
+template <bool B16, bool CAP, int PER> hipError_t go_verify(const VerifyArgs &a, hipStream_t s) {
+    const uint64_t seqs = a.n_seqs, chunks = a.chunks;
+    hipError_t e = start(k_verify_stats<B16, CAP, PER>, seqs * (a.max_drafts + 1) * chunks, VF_THREADS, s, a);
+    if (e == hipSuccess) e = start(k_verify_decide<B16, CAP, PER>, a.k > 0.0 ? seqs * chunks : seqs, VF_THREADS, s, a);
+    if (e == hipSuccess && a.k > 0.0) e = start(k_verify_draw<B16, CAP, PER>, seqs, VF_THREADS, s, a);
+    return e;
 }
-
-template <bool B16> void go_verify(const VerifyArgs &a, int per, hipStream_t s) {
-    if (a.cap > 0.0) { if (per == 4) go_verify<B16, true, 4>(a, s); else go_verify<B16, true, 16>(a, s); }
-    else { if (per == 4) go_verify<B16, false, 4>(a, s); else go_verify<B16, false, 16>(a, s); }
+template <bool B16> hipError_t go_verify(const VerifyArgs &a, int per, hipStream_t s) {
+    if (a.cap > 0.0) return per == 4 ? go_verify<B16, true, 4>(a, s) : go_verify<B16, true, 16>(a, s);
+    return per == 4 ? go_verify<B16, false, 4>(a, s) : go_verify<B16, false, 16>(a, s);
 }
 
 }  // namespace
@@ -191,11 +196,11 @@ int hipdec_rope_append_paged(const hipdec_rope *rope, const hipdec_paged_cache *
     const int passes = (a.heads + 2 * a.kv_heads + per_pass - 1) / per_pass;
     a.parts = rows->n_rows * passes <= 4 * kCus ? passes : 1;
     const uint64_t grid = rows->n_rows * a.parts;
+    if (!grid_fits(grid, ROPE_THREADS)) return refuse(me, "n_rows out of range");
     const bool rb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;
     hipStream_t s = (hipStream_t)stream;
-    if (rb) { if (cb) go_rope<true, true>(a, wide, (unsigned)grid, s); else go_rope<true, false>(a, wide, (unsigned)grid, s); }
-    else { if (cb) go_rope<false, true>(a, wide, (unsigned)grid, s); else go_rope<false, false>(a, wide, (unsigned)grid, s); }
-    return launched(me);
+    if (rb) return launched(me, cb ? go_rope<true, true>(a, wide, grid, s) : go_rope<true, false>(a, wide, grid, s));
+    return launched(me, cb ? go_rope<false, true>(a, wide, grid, s) : go_rope<false, false>(a, wide, grid, s));
 }
 
 int hipdec_attention_paged_workspace(uint64_t n_rows, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint64_t max_len,
@@ -240,21 +245,19 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
 
     const int g = (int)(rows->heads / cache->kv_heads), tiles = (g + 15) / 16;
     const uint64_t grid = rows->n_rows * cache->kv_heads * tiles * p.splits, joins = rows->n_rows * rows->heads;
-    if (grid > 0x7fffffffu || joins > 0x7fffffffu) return refuse(me, "n_rows * heads * max_len out of range");
+    if (!grid_fits(grid, 512) || !grid_fits(joins, 256)) return refuse(me, "n_rows * heads * max_len out of range");
     float *po = (float *)d_workspace;
     PagedAttn a{view(*cache), rows->d_q, rows->d_out, rows->q_stride, rows->out_stride, rows->d_lens, rows->d_seqs, (int)rows->heads,
                 g, tiles, (int)(rows->max_len < slots ? rows->max_len : slots), p.chunk, p.splits,
                 rows->scale * 1.44269504088896340736f, po, po + rows->n_rows * rows->heads * p.splits * cache->hd};
     const bool qb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;
-    const unsigned nj = (unsigned)joins;
     hipStream_t s = (hipStream_t)stream;
     switch (cache->hd) {
-    case 64: go_attention<64>(qb, cb, a, (unsigned)grid, nj, s); break;
-    case 128: go_attention<128>(qb, cb, a, (unsigned)grid, nj, s); break;
-    case 192: go_attention<192>(qb, cb, a, (unsigned)grid, nj, s); break;
-    default: go_attention<256>(qb, cb, a, (unsigned)grid, nj, s); break;
+    case 64: return launched(me, go_attention<64>(qb, cb, a, grid, joins, s));
+    case 128: return launched(me, go_attention<128>(qb, cb, a, grid, joins, s));
+    case 192: return launched(me, go_attention<192>(qb, cb, a, grid, joins, s));
+    default: return launched(me, go_attention<256>(qb, cb, a, grid, joins, s));
     }
-    return launched(me);
 }
 
 int hipdec_verify_drafts_workspace(uint64_t n_seqs, uint32_t max_drafts, uint32_t vocab, uint64_t *out_bytes) {
@@ -284,7 +287,7 @@ int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t wor
     const uint64_t need = verify_bytes(d->n_seqs, d->max_drafts, c.n);
     if (!d_workspace || workspace_bytes < need || !aligned16(d_workspace))
         return refuse(me, "workspace missing, too small (hipdec_verify_drafts_workspace) or not 16-byte aligned");
-    if (rows * c.n > 0x7fffffffu) return refuse(me, "n_seqs * max_drafts * vocab out of range");
+    if (!grid_fits(rows * c.n, VF_THREADS)) return refuse(me, "n_seqs * max_drafts * vocab out of range");
     if ((bad = wrong_place({d->d_logits, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms, d->d_tokens, d->d_accepted,
                             d_workspace}, stream)))
         return refuse(me, bad);
@@ -295,8 +298,7 @@ int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t wor
                        (int)d->n_seqs, (int)d->max_drafts, (int)d->vocab, c.n, greedy ? 0.0 : log2e / (double)d->temperature,
                        cap, cap > 0.0 ? 2.0 * log2e / cap : 0.0, st, (double *)(places + d->n_seqs), places, d->d_tokens, d->d_accepted};
     hipStream_t s = (hipStream_t)stream;
-    if (d->dtype == HIPDEC_ROWS_BF16) go_verify<true>(a, c.per, s); else go_verify<false>(a, c.per, s);
-    return launched(me);
+    return launched(me, d->dtype == HIPDEC_ROWS_BF16 ? go_verify<true>(a, c.per, s) : go_verify<false>(a, c.per, s));
 }
 
 }  // extern "C"

@@ -37,6 +37,7 @@ EXPORTS = [
     "hipdec_debug_gemm_plan",
     "hipdec_rope_frequencies", "hipdec_rope_append_paged", "hipdec_attention_paged_workspace", "hipdec_attention_paged",
     "hipdec_verify_drafts_workspace", "hipdec_verify_drafts",
+    "hipdec_requests_open", "hipdec_requests_admit", "hipdec_requests_release", "hipdec_requests_len", "hipdec_requests_step",
 ]
 
 
@@ -151,6 +152,12 @@ def load_library(path=None):
     lib.hipdec_attention_paged_workspace.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64, u64p]
     lib.hipdec_attention_paged.argtypes = [C.POINTER(PagedCache), C.POINTER(_AttentionRows), C.c_void_p, C.c_uint64, C.c_void_p]
     lib.hipdec_verify_drafts_workspace.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32, u64p]
+    lib.hipdec_requests_open.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32]
+    lib.hipdec_requests_admit.argtypes = [C.c_void_p, C.c_uint32]
+    lib.hipdec_requests_release.argtypes = [C.c_void_p, C.c_uint32]
+    lib.hipdec_requests_len.argtypes = [C.c_void_p, C.c_uint32, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]
+    lib.hipdec_requests_step.argtypes = [C.c_void_p, C.c_size_t, u32p, u32p, C.c_uint32, u32p, u32p, fp, fp, C.c_float,
+                                         C.c_float, u32p, u32p, fp]
     lib.hipdec_verify_drafts.argtypes = [C.POINTER(_Drafts), C.c_void_p, C.c_uint64, C.c_void_p]
     szp = C.POINTER(C.c_size_t)
     lib.hipdec_batch_begin.argtypes = [C.c_void_p, C.c_size_t]
@@ -669,6 +676,42 @@ class HipDecodeModel:
         self._chk(self._lib.hipdec_materialize_current_logits_block_batch(self._h, row, block_idx, softcap, _fptr(out),
                                                                           cap, C.byref(valid)))
         return out[:valid.value]
+
+    # ---- requests of their own prompts stepped together over a paged cache
+    def requests_open(self, page_size, n_pages, max_seqs):
+        self._chk(self._lib.hipdec_requests_open(self._h, page_size, n_pages, max_seqs))
+
+    def requests_admit(self, seq):
+        self._chk(self._lib.hipdec_requests_admit(self._h, seq))
+
+    def requests_release(self, seq):
+        self._chk(self._lib.hipdec_requests_release(self._h, seq))
+
+    def requests_len(self, seq):
+        """(positions the sequence holds, free pages of the pool)"""
+        n, free = C.c_size_t(), C.c_size_t()
+        self._chk(self._lib.hipdec_requests_len(self._h, seq, C.byref(n), C.byref(free)))
+        return n.value, free.value
+
+    def requests_step(self, seqs, tokens, drafts=None, n_drafts=None, draft_probs=None, uniforms=None, temperature=0.0,
+                      softcap=0.0, logits=False):
+        """(tokens[n][K + 1], accepted[n]), with logits=True also the raw logits [n][K + 1][vocab]; drafts [n][K]."""
+        u32p = C.POINTER(C.c_uint32)
+        u32 = lambda a: None if a is None else np.ascontiguousarray(a, dtype=np.uint32)  # noqa: E731
+        f32 = lambda a: None if a is None else np.ascontiguousarray(a, dtype=np.float32)  # noqa: E731
+        ptr = lambda a, t: None if a is None else a.ctypes.data_as(t)  # noqa: E731
+        seqs, tokens, drafts, n_drafts, draft_probs, uniforms = u32(seqs), u32(tokens), u32(drafts), u32(n_drafts), f32(draft_probs), f32(uniforms)
+        n, k = seqs.size, 0 if drafts is None else drafts.shape[1]
+        for a, shape in ((tokens, (n,)), (drafts, (n, k)), (n_drafts, (n,)), (draft_probs, (n, k, self.cfg.vocab)), (uniforms, (n, k + 1))):
+            if a is not None and a.shape != shape:
+                raise ValueError("expected an array of shape %s, got %s" % (shape, a.shape))
+        out, acc = np.empty((n, k + 1), np.uint32), np.empty(n, np.uint32)
+        lg = np.empty((n, k + 1, self.cfg.vocab), np.float32) if logits else None
+        self._chk(self._lib.hipdec_requests_step(self._h, n, ptr(seqs, u32p), ptr(tokens, u32p), k, ptr(n_drafts, u32p),
+                                                 ptr(drafts, u32p), ptr(draft_probs, C.POINTER(C.c_float)),
+                                                 ptr(uniforms, C.POINTER(C.c_float)), temperature, softcap, ptr(out, u32p),
+                                                 ptr(acc, u32p), ptr(lg, C.POINTER(C.c_float))))
+        return (out, acc, lg) if logits else (out, acc)
 
     def last_device_ms(self):
         ms = C.c_float()
