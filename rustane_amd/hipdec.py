@@ -305,10 +305,6 @@ class _Drafts(C.Structure):
                 ("d_tokens", C.c_void_p), ("d_accepted", C.c_void_p)]
 
 
-def _first(*values):
-    return next(v for v in values if v is not None)
-
-
 def _op_chk(lib, rc):
     if rc != OK:
         raise HipDecodeError(rc, (lib.hipdec_last_error(None) or b"").decode())
@@ -328,12 +324,14 @@ def rope_append_paged(rope, cache, q, k, v, q_out, positions, n_rows, heads, dty
                       row_stride=None, q_stride=None, k_stride=None, v_stride=None, q_out_stride=None, stream=None):
     """hipdec_rope_append_paged.  Strides in elements; row_stride stands for those of q, k and v where the three lie in
     one row (a fused projection); left out, rows are dense."""
-    lib = load_library()
-    wide, kv_wide = heads * cache.hd, cache.kv_heads * cache.hd
-    rows = _NewRows(q, k, v, q_out, dtype, heads, n_rows, _first(q_stride, row_stride, wide),
-                    _first(k_stride, row_stride, kv_wide), _first(v_stride, row_stride, kv_wide), _first(q_out_stride, wide),
-                    positions, slots, seqs)
-    _op_chk(lib, lib.hipdec_rope_append_paged(C.byref(rope), C.byref(cache), C.byref(rows), stream))
+    lib = _LIB or load_library()
+    hd = cache.hd
+    wide, kv_wide = (heads * hd, cache.kv_heads * hd) if row_stride is None else (row_stride, row_stride)
+    rc = lib.hipdec_rope_append_paged(rope, cache, _NewRows(
+        q, k, v, q_out, dtype, heads, n_rows, wide if q_stride is None else q_stride, kv_wide if k_stride is None else k_stride,
+        kv_wide if v_stride is None else v_stride, heads * hd if q_out_stride is None else q_out_stride, positions, slots, seqs), stream)
+    if rc:
+        _op_chk(lib, rc)
 
 
 def attention_paged_workspace(n_rows, heads, kv_heads, hd, max_len):
@@ -346,11 +344,14 @@ def attention_paged_workspace(n_rows, heads, kv_heads, hd, max_len):
 def attention_paged(cache, q, out, lens, n_rows, heads, max_len, dtype=RowDtype.F32, scale=None, seqs=None, q_stride=None,
                     out_stride=None, workspace=None, workspace_bytes=0, stream=None):
     """hipdec_attention_paged; scale: 1 / sqrt(hd) if left out, strides in elements (dense rows if left out)."""
-    lib = load_library()
-    rows = _AttentionRows(q, out, dtype, heads, n_rows, _first(q_stride, heads * cache.hd),
-                          _first(out_stride, heads * cache.hd), lens,
-                          seqs, max_len, max(cache.hd, 1) ** -0.5 if scale is None else scale)
-    _op_chk(lib, lib.hipdec_attention_paged(C.byref(cache), C.byref(rows), workspace, workspace_bytes, stream))
+    lib = _LIB or load_library()
+    hd = cache.hd
+    wide = heads * hd
+    rc = lib.hipdec_attention_paged(cache, _AttentionRows(
+        q, out, dtype, heads, n_rows, wide if q_stride is None else q_stride, wide if out_stride is None else out_stride, lens, seqs,
+        max_len, (hd or 1) ** -0.5 if scale is None else scale), workspace, workspace_bytes, stream)
+    if rc:
+        _op_chk(lib, rc)
 
 
 def verify_drafts_workspace(n_seqs, max_drafts, vocab):
@@ -364,10 +365,13 @@ def verify_drafts(logits, drafts, uniforms, tokens, accepted, n_seqs, max_drafts
                   softcap=0.0, n_drafts=None, draft_probs=None, row_stride=None, prob_stride=None, workspace=None,
                   workspace_bytes=0, stream=None):
     """hipdec_verify_drafts; strides in elements (dense rows if left out)."""
-    lib = load_library()
-    d = _Drafts(logits, dtype, vocab, n_seqs, max_drafts, temperature, softcap, _first(row_stride, vocab),
-                _first(prob_stride, vocab), drafts, n_drafts, draft_probs, uniforms, tokens, accepted)
-    _op_chk(lib, lib.hipdec_verify_drafts(C.byref(d), workspace, workspace_bytes, stream))
+    lib = _LIB or load_library()
+    rc = lib.hipdec_verify_drafts(_Drafts(
+        logits, dtype, vocab, n_seqs, max_drafts, temperature, softcap, vocab if row_stride is None else row_stride,
+        vocab if prob_stride is None else prob_stride, drafts, n_drafts, draft_probs, uniforms, tokens, accepted), workspace,
+        workspace_bytes, stream)
+    if rc:
+        _op_chk(lib, rc)
 
 
 def calibration_copy(nbytes, reps=1):
