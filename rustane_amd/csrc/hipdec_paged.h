@@ -252,16 +252,16 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
                 } else {
                     const float4 x = *(const float4 *)((const float *)a.q + i), y = *(const float4 *)((const float *)a.q + i + 4);
                     float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                    // 24 bits in three parts of 8, each the upper half of what is left: exact.  (An infinity leaves NaN in
+                    // the second part, as its scores would in the softmax.)
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) {
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint32_t b0 = f32_to_bf16_rne(f[2 * e]), b1 = f32_to_bf16_rne(f[2 * e + 1]);
-                            w[e] = b0 | b1 << 16;
-                            // (an infinity stays in the first part)
-                            f[2 * e] = (b0 & 0x7f80u) == 0x7f80u ? 0.0f : f[2 * e] - bf16_to_f32(b0);
-                            f[2 * e + 1] = (b1 & 0x7f80u) == 0x7f80u ? 0.0f : f[2 * e + 1] - bf16_to_f32(b1);
+                            w[e] = __builtin_amdgcn_perm(__float_as_uint(f[2 * e + 1]), __float_as_uint(f[2 * e]), 0x07060302u);
+                            f[2 * e] -= __uint_as_float(w[e] << 16);
+                            f[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
                         }
                         qr[p * KQ + j] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
@@ -329,26 +329,24 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
         pg_f4 s[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            s[t] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
-            pg_f4 other = s[t];                              // (fp32: two sums, half the chain and less rounding)
+            // sums of their own for each part of the queries (fp32 cache: two): short chains, and the small ones added first
+            pg_f4 sum[3] = {};
 #pragma unroll
             for (int j = 0; j < KQ; ++j) {
                 if (CB) {
 #pragma unroll
-                    for (int p = PARTS - 1; p >= 0; --p)
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pg_bf8, x.k[t][j]),
-                                                                       __builtin_bit_cast(pg_bf8, qr[p * KQ + j]), s[t], 0, 0, 0);
+                    for (int p = 0; p < PARTS; ++p)
+                        sum[p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pg_bf8, x.k[t][j]),
+                                                                         __builtin_bit_cast(pg_bf8, qr[p * KQ + j]), sum[p], 0, 0, 0);
                 } else {
                     const pg_u4 kw = x.k[t][j];
                     const uint32_t qw[4] = {qr[j].x, qr[j].y, qr[j].z, qr[j].w};
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e]), __uint_as_float(qw[e]), s[t], 0, 0, 0);
-                        other = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e + 1]), __uint_as_float(qw[e + 1]), other, 0, 0, 0);
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        sum[e % 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e]), __uint_as_float(qw[e]), sum[e % 2], 0, 0, 0);
                 }
             }
-            if (!CB) s[t] += other;
+            s[t] = CB && PARTS == 1 ? sum[0] : CB ? sum[0] + (sum[1] + sum[2]) : sum[0] + sum[1];
         }
         const bool more = b + WAVES < blocks;
         bool gaps = false;
