@@ -15,6 +15,7 @@
 
 #define VF_THREADS 256
 #define VF_WAVES (VF_THREADS / WAVE)
+#define VF_DECIDE 512                                        // threads of the deciding kernel
 
 struct VfStat { double sum; float top; uint32_t arg; };      // of one chunk of one row: max logit, the sum of weights (T > 0) or the maximum's first index (T = 0; else 0xffffffff)
 struct VfPlace { double inv; float top; int kept; };         // where a sequence's next token is drawn: 1 / the row's sum (0: nothing to draw), its maximum
@@ -42,22 +43,22 @@ template <bool B16> __device__ __forceinline__ float vf_logit(const VerifyArgs &
     const float x = B16 ? bf16_to_f32(((const uint16_t *)a.logits)[at]) : ((const float *)a.logits)[at];
     return fminf(x == x ? x : -INFINITY, 3.4028235e38f);     // a NaN is no possible token; infinite ones share the whole
 }
-// PER logits of a thread: those of its chunk, VF_THREADS apart, or neighbours; -inf behind the vocabulary
-template <bool B16, int PER, bool NEAR> __device__ __forceinline__ void vf_logits(const VerifyArgs &a, long long row, int chunk, float *x) {
-    const int first = chunk * PER * VF_THREADS;
-    const bool inside = first + PER * VF_THREADS <= a.vocab;
+// PER logits of a thread: those of its chunk, THREADS apart, or neighbours; -inf behind the vocabulary
+template <bool B16, int PER, bool NEAR, int THREADS = VF_THREADS> __device__ __forceinline__ void vf_logits(const VerifyArgs &a, long long row, int chunk, float *x) {
+    const int first = chunk * PER * THREADS;
+    const bool inside = first + PER * THREADS <= a.vocab;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int at = NEAR ? first + (int)threadIdx.x * PER + i : first + i * VF_THREADS + (int)threadIdx.x;
+        const int at = NEAR ? first + (int)threadIdx.x * PER + i : first + i * THREADS + (int)threadIdx.x;
         x[i] = inside || at < a.vocab ? vf_logit<B16>(a, row, at) : -INFINITY;
     }
 }
 // the draft's probabilities of the same tokens
-template <int PER, bool NEAR> __device__ __forceinline__ void vf_guess(const VerifyArgs &a, long long draft, int chunk, float *q) {
-    const int first = chunk * PER * VF_THREADS, d = a.drafts[draft];
+template <int PER, bool NEAR, int THREADS = VF_THREADS> __device__ __forceinline__ void vf_guess(const VerifyArgs &a, long long draft, int chunk, float *q) {
+    const int first = chunk * PER * THREADS, d = a.drafts[draft];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int at = NEAR ? first + (int)threadIdx.x * PER + i : first + i * VF_THREADS + (int)threadIdx.x;
+        const int at = NEAR ? first + (int)threadIdx.x * PER + i : first + i * THREADS + (int)threadIdx.x;
         q[i] = !a.probs ? d == at ? 1.0f : 0.0f : at < a.vocab ? a.probs[draft * a.prob_stride + at] : 0.0f;
     }
 }
@@ -102,11 +103,7 @@ template <bool CAP, bool EXACT_ZERO> __device__ __forceinline__ double vf_weight
 // max(p - q, 0), a NaN in q leaves 0.  (One fused operation wherever it is taken: a chunk whose sum is above 0 holds a
 // token that is.)
 __device__ __forceinline__ double vf_rest(double weight, double inv, float q) { return fmax(fma(weight, inv, -(double)q), 0.0); }
-__device__ __forceinline__ double vf_wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
-    return v;
-}
+__device__ __forceinline__ double vf_wave_sum(double v) { return wave_read_f64(wave_scan_f64(v), 63); }
 
 // The statistics of every row that a sequence's drafts reach, one workgroup per chunk of PER logits a thread.
 template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_stats(VerifyArgs a) {
@@ -127,7 +124,7 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
     if (a.k > 0.0) {
 #pragma unroll
         for (int i = 1; i < PER; ++i) top = fmaxf(top, x[i]);
-        top = wave_max(top);
+        top = wave_max_dpp(top);
         if (lane == 0) st[wave] = top;
         __syncthreads();
         top = fmaxf(fmaxf(st[0], st[1]), fmaxf(st[2], st[3]));
@@ -153,11 +150,11 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
     if (tid == 0) a.stats[(size_t)row * a.chunks + chunk] = VfStat{sum, top, arg};
 }
 
-// The decision, by every workgroup of the sequence for itself (a wave per draft, all of them at once up to four), then
+// The decision, by every workgroup of the sequence for itself (a wave per row, all of them at once up to seven drafts), then
 // the workgroup's chunk of max(p - q, 0) where a draft was not kept.  The first chunk's workgroup writes what is known
 // by now: the kept drafts and, where T = 0 or nothing is possible, the next token.
-template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_decide(VerifyArgs a) {
-    __shared__ double s_inv[256], ss[VF_WAVES];              // of each row (max_drafts <= 255)
+template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_DECIDE) void k_verify_decide(VerifyArgs a) {
+    __shared__ double s_inv[256], ss[VF_DECIDE / WAVE];      // of each row (max_drafts <= 255)
     __shared__ float s_top[256];
     __shared__ uint32_t s_arg[256];
     __shared__ int s_kept;
@@ -166,7 +163,7 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
     const int n = vf_drafts(a, s);
     if (tid == 0) s_kept = n;
     __syncthreads();
-    for (int i = wave; i <= n; i += VF_WAVES) {
+    for (int i = wave; i <= n; i += VF_DECIDE / WAVE) {
         const long long row = (long long)s * (K + 1) + i;
         const int d = i < n ? a.drafts[(size_t)s * K + i] : -1;
         const VfStat *st = a.stats + (size_t)row * a.chunks;
@@ -182,7 +179,7 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
         for (int j = 0; j < 4; ++j) if (better(mine[j].top, mine[j].arg, top, arg)) { top = mine[j].top; arg = mine[j].arg; }
         double sum = 0.0, ztop = 0.0;
         if (a.k > 0.0) {
-            top = wave_max(top);
+            top = wave_max_dpp(top);
             ztop = vf_capped<CAP>(a, top);
 #pragma unroll
             for (int j = 0; j < 4; ++j) if (64 * j < a.chunks) sum += mine[j].sum * vf_weight<CAP, true>(a, mine[j].top, ztop);
@@ -204,42 +201,37 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
     if (part == 0) {
         uint32_t *out = a.tokens + (size_t)s * (K + 1);
         const bool known = !(a.k > 0.0) || inv == 0.0;       // (the index of a row without a possible token is 0xffffffff)
-        for (int i = tid; i <= K; i += VF_THREADS)
+        for (int i = tid; i <= K; i += VF_DECIDE)
             if (i != kept || known) out[i] = i < kept ? (uint32_t)a.drafts[(size_t)s * K + i] : i == kept ? s_arg[kept] : 0xffffffffu;
         if (tid == 0) { a.accepted[s] = kept; a.places[s] = VfPlace{inv, top, kept}; }
     }
     if (kept == n || !(a.k > 0.0)) return;                   // behind the last draft the statistics hold the sums
     const long long row = (long long)s * (K + 1) + kept, dr = (long long)s * K + kept;
     const double ztop = vf_capped<CAP>(a, top);
-    float x[PER], q[PER];
-    vf_logits<B16, PER, false>(a, row, part, x);
-    vf_guess<PER, false>(a, dr, part, q);
+    constexpr int MINE = PER * VF_THREADS / VF_DECIDE;
+    float x[MINE], q[MINE];
+    vf_logits<B16, MINE, false, VF_DECIDE>(a, row, part, x);
+    vf_guess<MINE, false, VF_DECIDE>(a, dr, part, q);
     double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) sum += vf_rest(vf_weight<CAP, true>(a, x[j], ztop), inv, q[j]);
+    for (int j = 0; j < MINE; ++j) sum += vf_rest(vf_weight<CAP, true>(a, x[j], ztop), inv, q[j]);
     sum = vf_wave_sum(sum);
     if (lane == 0) ss[wave] = sum;
     __syncthreads();
-    if (tid == 0) a.sums[(size_t)s * a.chunks + part] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+    if (tid == 0) a.sums[(size_t)s * a.chunks + part] = ((ss[0] + ss[1]) + (ss[2] + ss[3])) + ((ss[4] + ss[5]) + (ss[6] + ss[7]));
 }
 
 // sum over the threads before this one and this one, and the whole (VF_WAVES values of LDS)
 __device__ __forceinline__ double vf_scan(double v, double *waves, double &before, double &whole) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double run = v;
-#pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) {
-        const double w = __shfl_up(run, o, WAVE);
-        if (lane >= o) run += w;
-    }
+    const double run = wave_scan_f64(v), up = wave_before_f64(run);
     if (lane == 63) waves[wave] = run;
-    const double up = __shfl_up(run, 1, WAVE);
     __syncthreads();
     double base = 0.0;
     whole = 0.0;
 #pragma unroll
     for (int k = 0; k < VF_WAVES; ++k) { if (k < wave) base += waves[k]; whole += waves[k]; }
-    before = base + (lane ? up : 0.0);
+    before = base + up;
     return base + run;
 }
 

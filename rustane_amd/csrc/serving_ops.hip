@@ -124,7 +124,7 @@ uint64_t verify_bytes(uint64_t n_seqs, uint32_t max_drafts, int chunks) {
 template <bool B16, bool CAP, int PER> hipError_t go_verify(const VerifyArgs &a, hipStream_t s) {
     const uint64_t seqs = a.n_seqs, chunks = a.chunks;
     hipError_t e = start(k_verify_stats<B16, CAP, PER>, seqs * (a.max_drafts + 1) * chunks, VF_THREADS, s, a);
-    if (e == hipSuccess) e = start(k_verify_decide<B16, CAP, PER>, a.k > 0.0 ? seqs * chunks : seqs, VF_THREADS, s, a);
+    if (e == hipSuccess) e = start(k_verify_decide<B16, CAP, PER>, a.k > 0.0 ? seqs * chunks : seqs, VF_DECIDE, s, a);
     if (e == hipSuccess && a.k > 0.0) e = start(k_verify_draw<B16, CAP, PER>, seqs, VF_THREADS, s, a);
     return e;
 }
@@ -287,7 +287,7 @@ int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t wor
     const uint64_t need = verify_bytes(d->n_seqs, d->max_drafts, c.n);
     if (!d_workspace || workspace_bytes < need || !aligned16(d_workspace))
         return refuse(me, "workspace missing, too small (hipdec_verify_drafts_workspace) or not 16-byte aligned");
-    if (!grid_fits(rows * c.n, VF_THREADS)) return refuse(me, "n_seqs * max_drafts * vocab out of range");
+    if (!grid_fits(rows * c.n, VF_THREADS) || !grid_fits(d->n_seqs * c.n, VF_DECIDE)) return refuse(me, "n_seqs * max_drafts * vocab out of range");
     if ((bad = wrong_place({d->d_logits, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms, d->d_tokens, d->d_accepted,
                             d_workspace}, stream)))
         return refuse(me, bad);

@@ -132,3 +132,15 @@ static inline void wave_argbest(float &v, uint32_t &i) {
         if (better(ov, oi, v, i)) { v = ov; i = oi; }
     }
 }
+// (the data-parallel moves of hipdec_common.h: running sum, a lane's value everywhere, the lane before's, the largest)
+static inline double wave_scan_f64(double v) {
+    const double mine = v;
+    double r = 0.0;
+    uint64_t all[64];
+    std::memcpy(all, emu::share(mine), sizeof all);
+    for (int i = 0; i <= emu::lane(); ++i) r += emu::of_bits<double>(all[i]);
+    return r;
+}
+static inline double wave_read_f64(double v, int lane) { return emu::from_lane(v, lane); }
+static inline double wave_before_f64(double v) { const double r = emu::from_lane(v, emu::lane() ? emu::lane() - 1 : 0); return emu::lane() ? r : 0.0; }
+static inline float wave_max_dpp(float v) { return wave_max(v); }

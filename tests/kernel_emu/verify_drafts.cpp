@@ -63,7 +63,7 @@ template <bool B16, bool CAP, int PER> static void run(const char *what, int voc
     const double log2e = 1.4426950408889634074;
     VerifyArgs a{lg, stride, stride, drafts, n, q, T > 0 ? u : nullptr, S, K, vocab, chunks, T > 0 ? log2e / T : 0.0, cap, cap > 0 ? 2 * log2e / cap : 0.0, st, sums, pl, tok, acc};
     emu::launch_grid([&] { k_verify_stats<B16, CAP, PER>(a); }, (unsigned)(rows * chunks), VF_THREADS);
-    emu::launch_grid([&] { k_verify_decide<B16, CAP, PER>(a); }, (unsigned)(T > 0 ? S * chunks : S), VF_THREADS);
+    emu::launch_grid([&] { k_verify_decide<B16, CAP, PER>(a); }, (unsigned)(T > 0 ? S * chunks : S), VF_DECIDE);
     if (T > 0) emu::launch_grid([&] { k_verify_draw<B16, CAP, PER>(a); }, (unsigned)S, VF_THREADS);
 
     int wrong = 0, kept_all = 0;
