@@ -235,53 +235,62 @@ __device__ __forceinline__ double vf_scan(double v, double *waves, double &befor
     return base + run;
 }
 
-// The draw: the chunk where the running sum passes the border (a thread per chunk), then the token inside it.
+// The draw: the chunk where the running sum passes the border (every wave for itself, four chunks a lane: no barrier
+// until the tokens), then the token inside it.
 template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_draw(VerifyArgs a) {
-    __shared__ double w1[VF_WAVES], w2[VF_WAVES], left;
-    __shared__ int hit_chunk, last_chunk, some, hit, last;
-    const int s = blockIdx.x, tid = threadIdx.x, K = a.max_drafts;
+    __shared__ double waves[VF_WAVES];
+    __shared__ int hit, last;
+    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, K = a.max_drafts;
     const int n = vf_drafts(a, s);
     const VfPlace at = a.places[s];
     const float u = a.u[(size_t)s * (K + 1) + K];
-    double mine = tid < a.chunks ? a.sums[(size_t)s * a.chunks + tid] : 0.0;
-    if (at.kept == n) mine = 0.0;                            // (nothing was written there)
+    double mine[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mine[j] = 4 * lane + j < a.chunks ? a.sums[(size_t)s * a.chunks + 4 * lane + j] : 0.0;
     if (at.inv == 0.0) return;                               // no possible token: already written
+    if (tid == 0) { hit = 0x7fffffff; last = -1; }
     const long long row = (long long)s * (K + 1) + at.kept, dr = (long long)s * K + at.kept;
     const double ztop = vf_capped<CAP>(a, at.top);
-    if (tid == 0) { hit_chunk = 0x7fffffff; last_chunk = -1; some = 0; hit = 0x7fffffff; last = -1; }
-    __syncthreads();
-    if (mine > 0.0) some = 1;
-    __syncthreads();
-    // all drafts kept, or the draft's distribution covers the target's everywhere: the target's own
-    const bool rest = some != 0;
-    if (!rest) {
-        const VfStat st = tid < a.chunks ? a.stats[(size_t)row * a.chunks + tid] : VfStat{0.0, -INFINITY, 0u};
-        mine = st.sum * vf_weight<CAP, true>(a, st.top, ztop) * at.inv;
-    }
-    double before, whole;
+    // all drafts kept (no sums were written then), or the draft's distribution covers the target's everywhere: the target's own
+    const bool rest = at.kept < n && __ballot(mine[0] > 0.0 || mine[1] > 0.0 || mine[2] > 0.0 || mine[3] > 0.0) != 0;
+    if (!rest)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const VfStat st = 4 * lane + j < a.chunks ? a.stats[(size_t)row * a.chunks + 4 * lane + j] : VfStat{0.0, -INFINITY, 0u};
+            mine[j] = st.sum * vf_weight<CAP, true>(a, st.top, ztop) * at.inv;
+        }
     // (a random number of 1 or more, or none: no running sum passes the border, and the last possible token it is)
-    const double run = vf_scan(mine, w1, before, whole), border = u < 1.0f ? (double)u * whole : INFINITY;
-    if (mine > 0.0) {
-        atomicMax(&last_chunk, tid);
-        if (run > border) atomicMin(&hit_chunk, tid);
+    double run = wave_scan_f64((mine[0] + mine[1]) + (mine[2] + mine[3]));
+    const double border = u < 1.0f ? (double)u * wave_read_f64(run, 63) : INFINITY;
+    run = wave_before_f64(run);
+    int in = -1, end = -1;                                   // chunk that passes the border; last chunk with any weight
+    double in_left = 0.0, end_left = 0.0;                    // ... and what of the border is left where it begins
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (mine[j] > 0.0) {
+            end = 4 * lane + j; end_left = border - run;
+            if (in < 0 && run + mine[j] > border) { in = end; in_left = end_left; }
+        }
+        run += mine[j];
     }
-    __syncthreads();
-    const int chunk = hit_chunk != 0x7fffffff ? hit_chunk : last_chunk;
-    if (tid == chunk) left = border - before;
-    const int i0 = (chunk * VF_THREADS + tid) * PER;         // in index order
+    const uint64_t ins = __ballot(in >= 0), ends = __ballot(end >= 0);
+    const int from = ins ? __ffsll((unsigned long long)ins) - 1 : 63 - __clzll((long long)ends);
+    const int chunk = __shfl(ins ? in : end, from, WAVE);
+    const double left = wave_read_f64(ins ? in_left : end_left, from);
+
     float x[PER], q[PER] = {};
     vf_logits<B16, PER, true>(a, row, chunk, x);
     if (rest) vf_guess<PER, true>(a, dr, chunk, q);
-    double w[PER];
-    mine = 0.0;
+    double w[PER], sum = 0.0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const double t = vf_weight<CAP, true>(a, x[j], ztop);
         w[j] = rest ? vf_rest(t, at.inv, q[j]) : t * at.inv;
-        mine += w[j];
+        sum += w[j];
     }
-    double r;
-    vf_scan(mine, w2, r, whole);                             // (its barrier also publishes `left`)
+    double r, whole;
+    vf_scan(sum, waves, r, whole);
+    const int i0 = (chunk * VF_THREADS + tid) * PER;         // in index order
     int my_hit = 0x7fffffff, my_last = -1;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
