@@ -13,9 +13,12 @@
 #pragma once
 #include "hipdec_common.h"
 
-#define VF_THREADS 256
-#define VF_WAVES (VF_THREADS / WAVE)
-#define VF_DECIDE 512                                        // threads of the deciding kernel
+// A chunk is what one wave takes: 64 * PER logits.  No barrier stands between a chunk's loads and its result, so the waves of
+// a CU drift apart and one's loads run under another's arithmetic (with a workgroup to a chunk and two barriers in it
+// 32 requests of 7 drafts took 30.2 us, so 24.5; the draw of one token 7.4 us, so 3.0).
+#define VF_STATS 256                                         // threads of the kernels: statistics,
+#define VF_DECIDE 512                                        // decision and rest
+#define VF_MAX_CHUNKS 256                                    // of a row: four a lane
 
 struct VfStat { double sum; float top; uint32_t arg; };      // of one chunk of one row: max logit, the sum of weights (T > 0) or the maximum's first index (T = 0; else 0xffffffff)
 struct VfPlace { double inv; float top; int kept; };         // where a sequence's next token is drawn: 1 / the row's sum (0: nothing to draw), its maximum
@@ -43,22 +46,22 @@ template <bool B16> __device__ __forceinline__ float vf_logit(const VerifyArgs &
     const float x = B16 ? bf16_to_f32(((const uint16_t *)a.logits)[at]) : ((const float *)a.logits)[at];
     return fminf(x == x ? x : -INFINITY, 3.4028235e38f);     // a NaN is no possible token; infinite ones share the whole
 }
-// PER logits of a thread: those of its chunk, THREADS apart, or neighbours; -inf behind the vocabulary
-template <bool B16, int PER, bool NEAR, int THREADS = VF_THREADS> __device__ __forceinline__ void vf_logits(const VerifyArgs &a, long long row, int chunk, float *x) {
-    const int first = chunk * PER * THREADS;
-    const bool inside = first + PER * THREADS <= a.vocab;
+// PER logits of a lane: those of its wave's chunk 64 apart, or neighbours; -inf behind the vocabulary
+template <bool B16, int PER, bool NEAR> __device__ __forceinline__ void vf_logits(const VerifyArgs &a, long long row, int chunk, float *x) {
+    const int first = chunk * PER * WAVE, lane = threadIdx.x & 63;
+    const bool inside = first + PER * WAVE <= a.vocab;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int at = NEAR ? first + (int)threadIdx.x * PER + i : first + i * THREADS + (int)threadIdx.x;
+        const int at = NEAR ? first + lane * PER + i : first + i * WAVE + lane;
         x[i] = inside || at < a.vocab ? vf_logit<B16>(a, row, at) : -INFINITY;
     }
 }
 // the draft's probabilities of the same tokens
-template <int PER, bool NEAR, int THREADS = VF_THREADS> __device__ __forceinline__ void vf_guess(const VerifyArgs &a, long long draft, int chunk, float *q) {
-    const int first = chunk * PER * THREADS, d = a.drafts[draft];
+template <int PER, bool NEAR> __device__ __forceinline__ void vf_guess(const VerifyArgs &a, long long draft, int chunk, float *q) {
+    const int first = chunk * PER * WAVE, lane = threadIdx.x & 63, d = a.drafts[draft];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int at = NEAR ? first + (int)threadIdx.x * PER + i : first + i * THREADS + (int)threadIdx.x;
+        const int at = NEAR ? first + lane * PER + i : first + i * WAVE + lane;
         q[i] = !a.probs ? d == at ? 1.0f : 0.0f : at < a.vocab ? a.probs[draft * a.prob_stride + at] : 0.0f;
     }
 }
@@ -105,14 +108,12 @@ template <bool CAP, bool EXACT_ZERO> __device__ __forceinline__ double vf_weight
 __device__ __forceinline__ double vf_rest(double weight, double inv, float q) { return fmax(fma(weight, inv, -(double)q), 0.0); }
 __device__ __forceinline__ double vf_wave_sum(double v) { return wave_read_f64(wave_scan_f64(v), 63); }
 
-// The statistics of every row that a sequence's drafts reach, one workgroup per chunk of PER logits a thread.
-template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_stats(VerifyArgs a) {
-    __shared__ float st[VF_WAVES];
-    __shared__ uint32_t si[VF_WAVES];
-    __shared__ double ss[VF_WAVES];
-    const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks;
-    const int s = row / (a.max_drafts + 1);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// The statistics of every row that a sequence's drafts reach, a wave per chunk.
+template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_STATS) void k_verify_stats(VerifyArgs a) {
+    const int per_row = (a.chunks + VF_STATS / WAVE - 1) / (VF_STATS / WAVE);
+    const int row = blockIdx.x / per_row, chunk = (int)(blockIdx.x % per_row) * (VF_STATS / WAVE) + (int)(threadIdx.x >> 6);
+    const int s = row / (a.max_drafts + 1), lane = threadIdx.x & 63;
+    if (chunk >= a.chunks) return;
     float x[PER];
     const bool unused = row - s * (a.max_drafts + 1) > vf_drafts(a, s);
     if (PER > 4 && unused) return;                           // (few logits are asked for without waiting for the draft's length)
@@ -125,41 +126,31 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
 #pragma unroll
         for (int i = 1; i < PER; ++i) top = fmaxf(top, x[i]);
         top = wave_max_dpp(top);
-        if (lane == 0) st[wave] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(st[0], st[1]), fmaxf(st[2], st[3]));
         const double ztop = vf_capped<CAP>(a, top);
 #pragma unroll
         for (int i = 0; i < PER; ++i) sum += vf_weight<CAP, false>(a, x[i], ztop);
-        sum = vf_wave_sum(sum);
-        if (lane == 0) ss[wave] = sum;
-        __syncthreads();
-        sum = top == -INFINITY ? 0.0 : (ss[0] + ss[1]) + (ss[2] + ss[3]);
+        sum = top == -INFINITY ? 0.0 : vf_wave_sum(sum);
     } else {
         top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (x[i] > top) { top = x[i]; arg = (uint32_t)((chunk * PER + i) * VF_THREADS + tid); }
+            if (x[i] > top) { top = x[i]; arg = (uint32_t)((chunk * PER + i) * WAVE + lane); }
         wave_argbest(top, arg);
-        if (lane == 0) { st[wave] = top; si[wave] = arg; }
-        __syncthreads();
-        top = st[0]; arg = si[0];
-#pragma unroll
-        for (int w = 1; w < VF_WAVES; ++w) if (better(st[w], si[w], top, arg)) { top = st[w]; arg = si[w]; }
     }
-    if (tid == 0) a.stats[(size_t)row * a.chunks + chunk] = VfStat{sum, top, arg};
+    if (lane == 0) a.stats[(size_t)row * a.chunks + chunk] = VfStat{sum, top, arg};
 }
 
 // The decision, by every workgroup of the sequence for itself (a wave per row, all of them at once up to seven drafts), then
-// the workgroup's chunk of max(p - q, 0) where a draft was not kept.  The first chunk's workgroup writes what is known
+// each wave's chunk of max(p - q, 0) where a draft was not kept.  The sequence's first workgroup writes what is known
 // by now: the kept drafts and, where T = 0 or nothing is possible, the next token.
 template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_DECIDE) void k_verify_decide(VerifyArgs a) {
-    __shared__ double s_inv[256], ss[VF_DECIDE / WAVE];      // of each row (max_drafts <= 255)
+    __shared__ double s_inv[256];                            // of each row (max_drafts <= 255)
     __shared__ float s_top[256];
     __shared__ uint32_t s_arg[256];
     __shared__ int s_kept;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.max_drafts;
-    const int part = a.k > 0.0 ? (int)(blockIdx.x % a.chunks) : 0, s = a.k > 0.0 ? (int)(blockIdx.x / a.chunks) : (int)blockIdx.x;
+    const int parts = a.k > 0.0 ? (a.chunks + VF_DECIDE / WAVE - 1) / (VF_DECIDE / WAVE) : 1;
+    const int s = blockIdx.x / parts, part = blockIdx.x % parts;
     const int n = vf_drafts(a, s);
     if (tid == 0) s_kept = n;
     __syncthreads();
@@ -168,7 +159,7 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_DECIDE) v
         const int d = i < n ? a.drafts[(size_t)s * K + i] : -1;
         const VfStat *st = a.stats + (size_t)row * a.chunks;
         float top = -INFINITY; uint32_t arg = 0xffffffffu;
-        VfStat mine[4];                                      // at most 256 chunks
+        VfStat mine[VF_MAX_CHUNKS / WAVE];
 #pragma unroll
         for (int j = 0; j < 4; ++j) mine[j] = lane + 64 * j < a.chunks ? st[lane + 64 * j] : VfStat{0.0, -INFINITY, 0xffffffffu};
         const bool real = (unsigned)d < (unsigned)a.vocab;
@@ -208,39 +199,22 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_DECIDE) v
     if (kept == n || !(a.k > 0.0)) return;                   // behind the last draft the statistics hold the sums
     const long long row = (long long)s * (K + 1) + kept, dr = (long long)s * K + kept;
     const double ztop = vf_capped<CAP>(a, top);
-    constexpr int MINE = PER * VF_THREADS / VF_DECIDE;
-    float x[MINE], q[MINE];
-    vf_logits<B16, MINE, false, VF_DECIDE>(a, row, part, x);
-    vf_guess<MINE, false, VF_DECIDE>(a, dr, part, q);
+    const int chunk = part * (VF_DECIDE / WAVE) + wave;
+    if (chunk >= a.chunks) return;
+    float x[PER], q[PER];
+    vf_logits<B16, PER, false>(a, row, chunk, x);
+    vf_guess<PER, false>(a, dr, chunk, q);
     double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < MINE; ++j) sum += vf_rest(vf_weight<CAP, true>(a, x[j], ztop), inv, q[j]);
+    for (int j = 0; j < PER; ++j) sum += vf_rest(vf_weight<CAP, true>(a, x[j], ztop), inv, q[j]);
     sum = vf_wave_sum(sum);
-    if (lane == 0) ss[wave] = sum;
-    __syncthreads();
-    if (tid == 0) a.sums[(size_t)s * a.chunks + part] = ((ss[0] + ss[1]) + (ss[2] + ss[3])) + ((ss[4] + ss[5]) + (ss[6] + ss[7]));
+    if (lane == 0) a.sums[(size_t)s * a.chunks + chunk] = sum;
 }
 
-// sum over the threads before this one and this one, and the whole (VF_WAVES values of LDS)
-__device__ __forceinline__ double vf_scan(double v, double *waves, double &before, double &whole) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const double run = wave_scan_f64(v), up = wave_before_f64(run);
-    if (lane == 63) waves[wave] = run;
-    __syncthreads();
-    double base = 0.0;
-    whole = 0.0;
-#pragma unroll
-    for (int k = 0; k < VF_WAVES; ++k) { if (k < wave) base += waves[k]; whole += waves[k]; }
-    before = base + up;
-    return base + run;
-}
-
-// The draw: the chunk where the running sum passes the border (every wave for itself, four chunks a lane: no barrier
-// until the tokens), then the token inside it.
-template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) void k_verify_draw(VerifyArgs a) {
-    __shared__ double waves[VF_WAVES];
-    __shared__ int hit, last;
-    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, K = a.max_drafts;
+// The draw, a wave per sequence: the chunk where the running sum passes the border (four chunks a lane), then the token
+// inside it.
+template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(WAVE) void k_verify_draw(VerifyArgs a) {
+    const int s = blockIdx.x, lane = threadIdx.x, K = a.max_drafts;
     const int n = vf_drafts(a, s);
     const VfPlace at = a.places[s];
     const float u = a.u[(size_t)s * (K + 1) + K];
@@ -248,7 +222,6 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
 #pragma unroll
     for (int j = 0; j < 4; ++j) mine[j] = 4 * lane + j < a.chunks ? a.sums[(size_t)s * a.chunks + 4 * lane + j] : 0.0;
     if (at.inv == 0.0) return;                               // no possible token: already written
-    if (tid == 0) { hit = 0x7fffffff; last = -1; }
     const long long row = (long long)s * (K + 1) + at.kept, dr = (long long)s * K + at.kept;
     const double ztop = vf_capped<CAP>(a, at.top);
     // all drafts kept (no sums were written then), or the draft's distribution covers the target's everywhere: the target's own
@@ -288,17 +261,15 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_THREADS) 
         w[j] = rest ? vf_rest(t, at.inv, q[j]) : t * at.inv;
         sum += w[j];
     }
-    double r, whole;
-    vf_scan(sum, waves, r, whole);
-    const int i0 = (chunk * VF_THREADS + tid) * PER;         // in index order
-    int my_hit = 0x7fffffff, my_last = -1;
+    double r = wave_before_f64(wave_scan_f64(sum));
+    const int i0 = chunk * PER * WAVE + lane * PER;          // in index order
+    int hit = -1, last = -1;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         r += w[j];
-        if (w[j] > 0.0) { my_last = i0 + j; if (r > left) my_hit = min(my_hit, i0 + j); }
+        if (w[j] > 0.0) { last = i0 + j; if (r > left && hit < 0) hit = last; }
     }
-    if (my_hit != 0x7fffffff) atomicMin(&hit, my_hit);
-    if (my_last >= 0) atomicMax(&last, my_last);
-    __syncthreads();
-    if (tid == 0) a.tokens[(size_t)s * (K + 1) + at.kept] = (uint32_t)(hit != 0x7fffffff ? hit : last);
+    const uint64_t hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
+    if (hits ? lane == __ffsll((unsigned long long)hits) - 1 : lane == 63 - __clzll((long long)lasts))
+        a.tokens[(size_t)s * (K + 1) + at.kept] = (uint32_t)(hits ? hit : last);
 }

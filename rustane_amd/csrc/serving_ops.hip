@@ -109,28 +109,30 @@ template <bool RB, bool CB> hipError_t go_rope(const RopeArgs &a, bool wide, uin
     return wide ? start(k_rope_append<RB, CB, 4>, grid, ROPE_THREADS, s, a) : start(k_rope_append<RB, CB, 1>, grid, ROPE_THREADS, s, a);
 }
 
-// Logits of a row per workgroup: 1024 where that makes few workgroups (the draw is latency: 18.1 us for five rows of
-// 32768 against 24, 33.8 us for 256 rows against 37), else 4096 (fewer reductions, and less of the statistics to read
-// back: 108 us for 384 rows of 131071 against 155).  At most 256 chunks: a thread each.
+// Logits of a row per wave: 256, 512 or 1024.  Few logits are latency, many are instructions, of which a chunk's maximum
+// and sum, and reading its statistics back, are a smaller part the more logits it has: 160 rows of 32768 21.3 / 23.6 /
+// 29.2 us, 512 rows 45.4 / 39.9 / 43.4, 256 rows of 131071 - / 81.5 / 78.7.  At most 256 chunks.
 struct Chunks { int per, n; };
 Chunks chunks_of(uint64_t rows, uint32_t vocab) {
-    const int per = rows * vocab <= (uint64_t)64 * kCus * 1024 ? 4 : 16;
-    return Chunks{per, (int)((vocab + per * VF_THREADS - 1) / (per * VF_THREADS))};
+    const uint64_t logits = rows * vocab;
+    int per = logits <= (6u << 20) ? 4 : logits <= (24u << 20) ? 8 : 16;
+    while ((vocab + per * WAVE - 1) / (per * WAVE) > VF_MAX_CHUNKS) per *= 2;
+    return Chunks{per, (int)((vocab + per * WAVE - 1) / (per * WAVE))};
 }
 uint64_t verify_bytes(uint64_t n_seqs, uint32_t max_drafts, int chunks) {
     return n_seqs * ((max_drafts + 1) * chunks * sizeof(VfStat) + chunks * sizeof(double) + sizeof(VfPlace));
 }
 
 template <bool B16, bool CAP, int PER> hipError_t go_verify(const VerifyArgs &a, hipStream_t s) {
-    const uint64_t seqs = a.n_seqs, chunks = a.chunks;
-    hipError_t e = start(k_verify_stats<B16, CAP, PER>, seqs * (a.max_drafts + 1) * chunks, VF_THREADS, s, a);
-    if (e == hipSuccess) e = start(k_verify_decide<B16, CAP, PER>, a.k > 0.0 ? seqs * chunks : seqs, VF_DECIDE, s, a);
-    if (e == hipSuccess && a.k > 0.0) e = start(k_verify_draw<B16, CAP, PER>, seqs, VF_THREADS, s, a);
+    const uint64_t seqs = a.n_seqs, few = (a.chunks + VF_STATS / WAVE - 1) / (VF_STATS / WAVE), more = (a.chunks + VF_DECIDE / WAVE - 1) / (VF_DECIDE / WAVE);
+    hipError_t e = start(k_verify_stats<B16, CAP, PER>, seqs * (a.max_drafts + 1) * few, VF_STATS, s, a);
+    if (e == hipSuccess) e = start(k_verify_decide<B16, CAP, PER>, a.k > 0.0 ? seqs * more : seqs, VF_DECIDE, s, a);
+    if (e == hipSuccess && a.k > 0.0) e = start(k_verify_draw<B16, CAP, PER>, seqs, WAVE, s, a);
     return e;
 }
 template <bool B16> hipError_t go_verify(const VerifyArgs &a, int per, hipStream_t s) {
-    if (a.cap > 0.0) return per == 4 ? go_verify<B16, true, 4>(a, s) : go_verify<B16, true, 16>(a, s);
-    return per == 4 ? go_verify<B16, false, 4>(a, s) : go_verify<B16, false, 16>(a, s);
+    if (a.cap > 0.0) return per == 4 ? go_verify<B16, true, 4>(a, s) : per == 8 ? go_verify<B16, true, 8>(a, s) : go_verify<B16, true, 16>(a, s);
+    return per == 4 ? go_verify<B16, false, 4>(a, s) : per == 8 ? go_verify<B16, false, 8>(a, s) : go_verify<B16, false, 16>(a, s);
 }
 
 }  // namespace
@@ -287,7 +289,7 @@ int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t wor
     const uint64_t need = verify_bytes(d->n_seqs, d->max_drafts, c.n);
     if (!d_workspace || workspace_bytes < need || !aligned16(d_workspace))
         return refuse(me, "workspace missing, too small (hipdec_verify_drafts_workspace) or not 16-byte aligned");
-    if (!grid_fits(rows * c.n, VF_THREADS) || !grid_fits(d->n_seqs * c.n, VF_DECIDE)) return refuse(me, "n_seqs * max_drafts * vocab out of range");
+    if (!grid_fits(rows * c.n, VF_STATS)) return refuse(me, "n_seqs * max_drafts * vocab out of range");
     if ((bad = wrong_place({d->d_logits, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms, d->d_tokens, d->d_accepted,
                             d_workspace}, stream)))
         return refuse(me, bad);

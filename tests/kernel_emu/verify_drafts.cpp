@@ -15,7 +15,7 @@ template <class T> static T *heap(size_t n) { return (T *)std::malloc(n * sizeof
 enum { PLAIN, ALL_IMPOSSIBLE, NAN_LOGITS, INF_LOGIT, COVERED, OUTSIDE, U_ZERO, U_ONE, NAN_PROBS, TIES, SPECIALS };
 
 template <bool B16, bool CAP, int PER> static void run(const char *what, int vocab, int K, float T, float cap, bool probs) {
-    const int S = SPECIALS, rows = S * (K + 1), chunks = (vocab + PER * VF_THREADS - 1) / (PER * VF_THREADS), stride = vocab + 3;
+    const int S = SPECIALS, rows = S * (K + 1), chunks = (vocab + PER * WAVE - 1) / (PER * WAVE), stride = vocab + 3;
     std::normal_distribution<float> nd(0.0f, 3.0f);
     std::uniform_real_distribution<float> ud(0.0f, 1.0f);
     void *lg = std::malloc((size_t)rows * stride * (B16 ? 2 : 4));
@@ -62,9 +62,9 @@ template <bool B16, bool CAP, int PER> static void run(const char *what, int voc
     std::memset(st, 0x7f, (size_t)rows * chunks * sizeof(VfStat)); std::memset(sums, 0x7f, (size_t)S * chunks * 8); std::memset(pl, 0x7f, S * sizeof(VfPlace));
     const double log2e = 1.4426950408889634074;
     VerifyArgs a{lg, stride, stride, drafts, n, q, T > 0 ? u : nullptr, S, K, vocab, chunks, T > 0 ? log2e / T : 0.0, cap, cap > 0 ? 2 * log2e / cap : 0.0, st, sums, pl, tok, acc};
-    emu::launch_grid([&] { k_verify_stats<B16, CAP, PER>(a); }, (unsigned)(rows * chunks), VF_THREADS);
-    emu::launch_grid([&] { k_verify_decide<B16, CAP, PER>(a); }, (unsigned)(T > 0 ? S * chunks : S), VF_DECIDE);
-    if (T > 0) emu::launch_grid([&] { k_verify_draw<B16, CAP, PER>(a); }, (unsigned)S, VF_THREADS);
+    emu::launch_grid([&] { k_verify_stats<B16, CAP, PER>(a); }, (unsigned)(rows * ((chunks + VF_STATS / WAVE - 1) / (VF_STATS / WAVE))), VF_STATS);
+    emu::launch_grid([&] { k_verify_decide<B16, CAP, PER>(a); }, (unsigned)(T > 0 ? S * ((chunks + VF_DECIDE / WAVE - 1) / (VF_DECIDE / WAVE)) : S), VF_DECIDE);
+    if (T > 0) emu::launch_grid([&] { k_verify_draw<B16, CAP, PER>(a); }, (unsigned)S, WAVE);
 
     int wrong = 0, kept_all = 0;
     std::vector<double> p(vocab), qq(vocab);
