@@ -312,8 +312,9 @@ int hipdec_sample_fullvocab_noalloc(const float *d_logits, size_t vocab, const f
  * calls, so a call can be recorded into a graph.  Workspaces are the caller's: one per call in flight (two
  * streams, or two graphs that may run at once, need one each).  Structs are read before the call returns.
  * Errors are reported through hipdec_last_error(NULL) on the calling thread; after a refusal
- * (HIPDEC_ERR_ARG, _UNSUPPORTED) nothing was enqueued.  Numbers in device memory cannot be checked on the host: what each call makes of those that are
- * out of range is said with it, and none leads outside the buffers described. */
+ * (HIPDEC_ERR_ARG, _UNSUPPORTED) nothing was enqueued.  Numbers in device memory cannot be checked on the host:
+ * what each call makes of those that are out of range is said with it, and none leads outside the buffers
+ * described. */
 
 typedef enum {               /* number format of rows and logits */
     HIPDEC_ROWS_F32 = 0,
@@ -384,7 +385,8 @@ int hipdec_rope_append_paged(const hipdec_rope *rope, const hipdec_paged_cache *
  * A row without a slot (length 0, a sequence that does not exist) gives zeros; slots whose page does not
  * exist are left out.  scale > 0.  hd: 64, 128, 192 or 256 (else HIPDEC_ERR_UNSUPPORTED); d_q, d_out and the
  * cache 16-byte aligned with strides that are multiples of 16 bytes.  d_workspace: at least
- * hipdec_attention_paged_workspace bytes for the same sizes and max_len, 16-byte aligned (may be NULL if that is 0). */
+ * hipdec_attention_paged_workspace bytes (which also serve fewer rows and any smaller max_len), 16-byte aligned
+ * (may be NULL if that is 0).  d_out may be d_q with the same stride, and must not overlap it otherwise. */
 typedef struct {
     const void *d_q;
     void *d_out;
@@ -400,19 +402,24 @@ int hipdec_attention_paged_workspace(uint64_t n_rows, uint32_t heads, uint32_t k
 int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attention_rows *rows, void *d_workspace,
                            uint64_t workspace_bytes, void *stream);
 
-/* Which of a sequence's drafted tokens the target model keeps, and the token behind them.  Row s * (max_drafts + 1) + i
- * of d_logits (at that many row_strides) holds the target's logits where draft i of sequence s stands, the row behind
- * the last draft those of the next token; d_n_drafts[s] (NULL: max_drafts; clamped to 0 .. max_drafts) drafts count.
- * With p = softmax(softcap(logits) / temperature) and q = the draft's probabilities (d_draft_probs row
- * s * max_drafts + i; NULL: certain of its token), draft i is kept while d_uniforms[s][i] * q(draft) < p(draft); where
- * it is not, the next token is drawn from max(p - q, 0) (from p if that is zero everywhere), behind the last kept
- * draft from p: the lowest index whose running sum exceeds d_uniforms[s][max_drafts] times the whole sum, both in 64
- * bits (a number of 1 or more, or a NaN: the last token with any probability).  temperature 0: p is certain of the largest logit (the lowest index of equals) and q of the draft, no random
- * number is used (d_uniforms may be NULL).  d_tokens[s][max_drafts + 1]: the kept drafts, the next token, then
- * 0xffffffff; d_accepted[s]: how many drafts were kept.  A draft outside the vocabulary is not kept; NaN logits are
- * impossible tokens, and so are those of -inf; a row of nothing else gives the next token 0xffffffff.  softcap <= 0:
- * none.  vocab <= 262144, max_drafts 0 .. 255.  d_workspace: at least hipdec_verify_drafts_workspace bytes, 16-byte
- * aligned. */
+/* Which of a sequence's drafted tokens the target model keeps, and the token behind them.  Row
+ * s * (max_drafts + 1) + i of d_logits (rows row_stride apart) holds the target's logits for the place of draft i of
+ * sequence s, the row behind its last draft those for the token after it; d_n_drafts[s] drafts count (NULL:
+ * max_drafts; clamped to 0 .. max_drafts).  With p = softmax(softcap(logits) / temperature) and q = the draft's own
+ * probabilities (d_draft_probs row s * max_drafts + i; NULL: certain of its token), draft i is kept while
+ *     d_uniforms[s][i] * q(draft) < p(draft),
+ * random numbers in [0, 1) that do not depend on the drafts.  At the first that is not kept the next token is drawn
+ * from max(p - q, 0) (from p where that is zero everywhere), behind the last draft from p: the lowest index whose
+ * running sum exceeds d_uniforms[s][max_drafts] times the whole sum (a number of 1 or more, or a NaN: the last token
+ * with any probability).  Exponentials and sums are 64 bits wide.  Kept and drawn tokens together then follow the
+ * target's distribution.
+ *   temperature 0: p is certain of the largest logit (the lowest index of equals), q of the draft, and no random
+ * number is used (d_uniforms may be NULL).
+ *   d_tokens[s][max_drafts + 1]: the kept drafts, the next token, then 0xffffffff; d_accepted[s]: how many drafts
+ * were kept.  A draft outside the vocabulary is not kept; logits that are NaN or -inf are impossible tokens, and a row
+ * of nothing else gives the next token 0xffffffff.  softcap <= 0: none.  vocab <= 262144, max_drafts 0 .. 255.
+ *   d_workspace: at least hipdec_verify_drafts_workspace bytes (which also serve fewer sequences, fewer drafts and a
+ * smaller vocabulary), 16-byte aligned. */
 typedef struct {
     const void *d_logits;
     uint32_t dtype, vocab;               /* hipdec_row_dtype */

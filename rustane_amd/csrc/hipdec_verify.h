@@ -41,30 +41,55 @@ struct VerifyArgs {
 __device__ __forceinline__ int vf_drafts(const VerifyArgs &a, int s) {
     return a.n_drafts ? min(max(a.n_drafts[s], 0), a.max_drafts) : a.max_drafts;
 }
-template <bool B16> __device__ __forceinline__ float vf_logit(const VerifyArgs &a, long long row, int i) {
-    const long long at = row * a.row_stride + i;
-    const float x = B16 ? bf16_to_f32(((const uint16_t *)a.logits)[at]) : ((const float *)a.logits)[at];
-    return fminf(x == x ? x : -INFINITY, 3.4028235e38f);     // a NaN is no possible token; infinite ones share the whole
+// stored logit as a number: a NaN is no possible token; infinite ones share the whole
+template <bool B16> __device__ __forceinline__ float vf_number(uint32_t raw) {
+    const float x = B16 ? bf16_to_f32(raw) : __uint_as_float(raw);
+    return fminf(x == x ? x : -INFINITY, 3.4028235e38f);
 }
-// PER logits of a lane: those of its wave's chunk 64 apart, or neighbours; -inf behind the vocabulary
+template <bool B16> __device__ __forceinline__ uint32_t vf_raw(const void *row, int i) {
+    return B16 ? ((const uint16_t *)row)[i] : ((const uint32_t *)row)[i];
+}
+template <bool B16> __device__ __forceinline__ const void *vf_row_of(const VerifyArgs &a, long long row) {
+    return B16 ? (const void *)((const uint16_t *)a.logits + row * a.row_stride) : (const void *)((const float *)a.logits + row * a.row_stride);
+}
+template <bool B16> __device__ __forceinline__ float vf_logit(const VerifyArgs &a, long long row, int i) {
+    return vf_number<B16>(vf_raw<B16>(vf_row_of<B16>(a, row), i));
+}
+// PER logits of a lane: those of its wave's chunk 64 apart, or neighbours; -inf behind the vocabulary.  (All of them are
+// asked for before the first is looked at; the chunk is the same for the whole wave, and so is the question whether it
+// ends inside the vocabulary: with the check
+// around every load they went one after the other: 256 rows of 131071 took 79 us, so 50.)
 template <bool B16, int PER, bool NEAR> __device__ __forceinline__ void vf_logits(const VerifyArgs &a, long long row, int chunk, float *x) {
-    const int first = chunk * PER * WAVE, lane = threadIdx.x & 63;
-    const bool inside = first + PER * WAVE <= a.vocab;
+    const int first = chunk * PER * WAVE, lane = threadIdx.x & 63, step = NEAR ? 1 : WAVE, mine = first + (NEAR ? lane * PER : lane);
+    const void *p = vf_row_of<B16>(a, row);
+    uint32_t raw[PER];
+    if (first + PER * WAVE <= a.vocab) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int at = NEAR ? first + lane * PER + i : first + i * WAVE + lane;
-        x[i] = inside || at < a.vocab ? vf_logit<B16>(a, row, at) : -INFINITY;
+        for (int i = 0; i < PER; ++i) raw[i] = vf_raw<B16>(p, mine + i * step);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[i] = vf_number<B16>(raw[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) raw[i] = vf_raw<B16>(p, min(mine + i * step, a.vocab - 1));
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[i] = mine + i * step < a.vocab ? vf_number<B16>(raw[i]) : -INFINITY;
     }
 }
 // the draft's probabilities of the same tokens
 template <int PER, bool NEAR> __device__ __forceinline__ void vf_guess(const VerifyArgs &a, long long draft, int chunk, float *q) {
-    const int first = chunk * PER * WAVE, lane = threadIdx.x & 63, d = a.drafts[draft];
+    const int lane = threadIdx.x & 63, step = NEAR ? 1 : WAVE, mine = chunk * PER * WAVE + (NEAR ? lane * PER : lane);
+    if (a.probs) {
+        const float *p = a.probs + draft * a.prob_stride;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int at = NEAR ? first + lane * PER + i : first + i * WAVE + lane;
-        q[i] = !a.probs ? d == at ? 1.0f : 0.0f : at < a.vocab ? a.probs[draft * a.prob_stride + at] : 0.0f;
+        for (int i = 0; i < PER; ++i) q[i] = p[min(mine + i * step, a.vocab - 1)];   // (behind the vocabulary the target has nothing)
+    } else {
+        const int d = a.drafts[draft];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) q[i] = d == mine + i * step ? 1.0f : 0.0f;
     }
 }
+// this thread's wave, known to be one number for the whole wave
+__device__ __forceinline__ int vf_wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
 // 2^y for -1021 <= y <= 1022: y = n + f with |f| <= 1/2, the series of 2^f = e^(f ln 2) up to its 11th power (the rest
 // is below 0.3466^12 / 12! = 7e-15 of it), scaled by 2^n in the exponent's bits.  n is read off the last bits of
@@ -111,7 +136,7 @@ __device__ __forceinline__ double vf_wave_sum(double v) { return wave_read_f64(w
 // The statistics of every row that a sequence's drafts reach, a wave per chunk.
 template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_STATS) void k_verify_stats(VerifyArgs a) {
     const int per_row = (a.chunks + VF_STATS / WAVE - 1) / (VF_STATS / WAVE);
-    const int row = blockIdx.x / per_row, chunk = (int)(blockIdx.x % per_row) * (VF_STATS / WAVE) + (int)(threadIdx.x >> 6);
+    const int row = blockIdx.x / per_row, chunk = (int)(blockIdx.x % per_row) * (VF_STATS / WAVE) + vf_wave();
     const int s = row / (a.max_drafts + 1), lane = threadIdx.x & 63;
     if (chunk >= a.chunks) return;
     float x[PER];
@@ -148,7 +173,7 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_DECIDE) v
     __shared__ float s_top[256];
     __shared__ uint32_t s_arg[256];
     __shared__ int s_kept;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.max_drafts;
+    const int tid = threadIdx.x, lane = tid & 63, wave = vf_wave(), K = a.max_drafts;
     const int parts = a.k > 0.0 ? (a.chunks + VF_DECIDE / WAVE - 1) / (VF_DECIDE / WAVE) : 1;
     const int s = blockIdx.x / parts, part = blockIdx.x % parts;
     const int n = vf_drafts(a, s);
@@ -161,11 +186,15 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_DECIDE) v
         float top = -INFINITY; uint32_t arg = 0xffffffffu;
         VfStat mine[VF_MAX_CHUNKS / WAVE];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mine[j] = lane + 64 * j < a.chunks ? st[lane + 64 * j] : VfStat{0.0, -INFINITY, 0xffffffffu};
+        for (int j = 0; j < 4; ++j) mine[j] = st[min(lane + 64 * j, a.chunks - 1)];
         const bool real = (unsigned)d < (unsigned)a.vocab;
-        const float x = real ? vf_logit<B16>(a, row, d) : -INFINITY;
-        const double q = real && a.k > 0.0 && a.probs ? (double)a.probs[((long long)s * K + i) * a.prob_stride + d] : 1.0;
-        const double u = a.k > 0.0 && i < n ? (double)a.u[(size_t)s * (K + 1) + i] : 0.0;
+        const int at = real ? d : 0;
+        const float logit = vf_logit<B16>(a, row, at), x = real ? logit : -INFINITY;
+        const bool sampled = a.k > 0.0 && i < n;
+        const double q = sampled && a.probs ? (double)a.probs[((long long)s * K + i) * a.prob_stride + at] : 1.0;
+        const double u = sampled ? (double)a.u[(size_t)s * (K + 1) + i] : 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (lane + 64 * j >= a.chunks) mine[j] = VfStat{0.0, -INFINITY, 0xffffffffu};
 #pragma unroll
         for (int j = 0; j < 4; ++j) if (better(mine[j].top, mine[j].arg, top, arg)) { top = mine[j].top; arg = mine[j].arg; }
         double sum = 0.0, ztop = 0.0;
@@ -220,7 +249,9 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(WAVE) void k
     const float u = a.u[(size_t)s * (K + 1) + K];
     double mine[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mine[j] = 4 * lane + j < a.chunks ? a.sums[(size_t)s * a.chunks + 4 * lane + j] : 0.0;
+    for (int j = 0; j < 4; ++j) mine[j] = a.sums[(size_t)s * a.chunks + min(4 * lane + j, a.chunks - 1)];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) if (4 * lane + j >= a.chunks) mine[j] = 0.0;
     if (at.inv == 0.0) return;                               // no possible token: already written
     const long long row = (long long)s * (K + 1) + at.kept, dr = (long long)s * K + at.kept;
     const double ztop = vf_capped<CAP>(a, at.top);
@@ -229,8 +260,8 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(WAVE) void k
     if (!rest)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const VfStat st = 4 * lane + j < a.chunks ? a.stats[(size_t)row * a.chunks + 4 * lane + j] : VfStat{0.0, -INFINITY, 0u};
-            mine[j] = st.sum * vf_weight<CAP, true>(a, st.top, ztop) * at.inv;
+            const VfStat st = a.stats[(size_t)row * a.chunks + min(4 * lane + j, a.chunks - 1)];
+            mine[j] = 4 * lane + j < a.chunks ? st.sum * vf_weight<CAP, true>(a, st.top, ztop) * at.inv : 0.0;
         }
     // (a random number of 1 or more, or none: no running sum passes the border, and the last possible token it is)
     double run = wave_scan_f64((mine[0] + mine[1]) + (mine[2] + mine[3]));
@@ -248,7 +279,7 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(WAVE) void k
     }
     const uint64_t ins = __ballot(in >= 0), ends = __ballot(end >= 0);
     const int from = ins ? __ffsll((unsigned long long)ins) - 1 : 63 - __clzll((long long)ends);
-    const int chunk = __shfl(ins ? in : end, from, WAVE);
+    const int chunk = __builtin_amdgcn_readlane(ins ? in : end, from);
     const double left = wave_read_f64(ins ? in_left : end_left, from);
 
     float x[PER], q[PER] = {};

@@ -90,6 +90,18 @@ Split split_of(uint64_t n_rows, uint32_t kv_heads, uint32_t g, uint64_t max_len)
     return Split{(int)per * 128, (int)((steps + per - 1) / per)};
 }
 
+// Workspace for n_rows rows and max_len, and for anything smaller in either: with u key-head tiles per row, rows * splits
+// is at most rows * steps / 8 where the 1024 keys decide, and rows * (2 CUs / (rows u) + 1) where the CUs do.
+uint64_t attention_bytes(uint64_t n_rows, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint64_t max_len) {
+    if (max_len <= 256 || !n_rows) return 0;
+    const uint64_t u = (uint64_t)kv_heads * ((heads / kv_heads + 15) / 16), steps = (max_len + 127) / 128;
+    uint64_t most = n_rows * ((steps + 7) / 8);
+    const uint64_t by_cus = (2 * kCus + u - 1) / u + n_rows;
+    if (most < by_cus) most = by_cus;
+    if (most > n_rows * steps) most = n_rows * steps;
+    return most * heads * (hd + 2) * sizeof(float);
+}
+
 template <int HD, bool QB, bool CB, bool FEW> hipError_t go_attention(const PagedAttn &a, uint64_t grid, uint64_t joins, hipStream_t s) {
     // (eight waves of the widest fp32 heads would not keep their registers)
     constexpr int WIDE = HD * (CB ? 2 : 4) <= 512 ? 8 : 4;
@@ -110,12 +122,12 @@ template <bool RB, bool CB> hipError_t go_rope(const RopeArgs &a, bool wide, uin
 }
 
 // Logits of a row per wave: 256, 512 or 1024.  Few logits are latency, many are instructions, of which a chunk's maximum
-// and sum, and reading its statistics back, are a smaller part the more logits it has: 160 rows of 32768 21.3 / 23.6 /
-// 29.2 us, 512 rows 45.4 / 39.9 / 43.4, 256 rows of 131071 - / 81.5 / 78.7.  At most 256 chunks.
+// and sum, and reading its statistics back, are a smaller part the more logits it has: 160 rows of 32768 17.2 / 16.6 /
+// 18.2 us, 512 rows 35.2 / 29.0 / 29.5, 256 rows of 131071 - / 53.5 / 49.9.  At most 256 chunks.
 struct Chunks { int per, n; };
 Chunks chunks_of(uint64_t rows, uint32_t vocab) {
     const uint64_t logits = rows * vocab;
-    int per = logits <= (6u << 20) ? 4 : logits <= (24u << 20) ? 8 : 16;
+    int per = logits <= (4u << 20) ? 4 : logits <= (12u << 20) ? 8 : 16;
     while ((vocab + per * WAVE - 1) / (per * WAVE) > VF_MAX_CHUNKS) per *= 2;
     return Chunks{per, (int)((vocab + per * WAVE - 1) / (per * WAVE))};
 }
@@ -211,8 +223,7 @@ int hipdec_attention_paged_workspace(uint64_t n_rows, uint32_t heads, uint32_t k
     if (!out_bytes) return refuse(me, "null argument");
     if (!heads || !kv_heads || heads % kv_heads || heads > 65536 || hd > kMaxHeadDim || n_rows > kMaxRows || max_len > kMaxLen)
         return refuse(me, "heads, hd, n_rows or max_len out of range");
-    const Split p = split_of(n_rows, kv_heads, heads / kv_heads, max_len);
-    *out_bytes = p.splits == 1 ? 0 : n_rows * heads * p.splits * (hd + 2) * sizeof(float);
+    *out_bytes = attention_bytes(n_rows, heads, kv_heads, hd, max_len);
     return HIPDEC_OK;
 }
 
@@ -226,7 +237,7 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
     if (rows->dtype > HIPDEC_ROWS_BF16) return refuse(me, "unknown dtype");
     if (!rows->heads || rows->heads % cache->kv_heads || rows->heads > 65536) return refuse(me, "heads must be a multiple of the cache's kv_heads");
     if (rows->n_rows > kMaxRows || rows->max_len > kMaxLen) return refuse(me, "n_rows or max_len out of range");
-    if (!(rows->scale > 0.0f) || !isfinite(rows->scale)) return refuse(me, "scale must be above 0");
+    if (!(rows->scale > 0.0f) || !isfinite(rows->scale * 1.44269504088896340736f)) return refuse(me, "scale must be above 0");
     if (cache->hd != 64 && cache->hd != 128 && cache->hd != 192 && cache->hd != 256)
         return hipdec_op_error(HIPDEC_ERR_UNSUPPORTED, me, "head dim must be 64, 128, 192 or 256");
     const int64_t wide = (int64_t)rows->heads * cache->hd;
@@ -266,7 +277,9 @@ int hipdec_verify_drafts_workspace(uint64_t n_seqs, uint32_t max_drafts, uint32_
     const char *me = "hipdec_verify_drafts_workspace";
     if (!out_bytes) return refuse(me, "null argument");
     if (max_drafts > kMaxDrafts || n_seqs > kMaxRows || !vocab || vocab > kMaxVocab) return refuse(me, "n_seqs, max_drafts or vocab out of range");
-    *out_bytes = verify_bytes(n_seqs, max_drafts, chunks_of(n_seqs * (max_drafts + 1), vocab).n);
+    // (the most chunks any smaller call makes of a row)
+    const uint32_t chunks = (vocab + 4 * WAVE - 1) / (4 * WAVE);
+    *out_bytes = verify_bytes(n_seqs, max_drafts, (int)(chunks < VF_MAX_CHUNKS ? chunks : VF_MAX_CHUNKS));
     return HIPDEC_OK;
 }
 

@@ -118,6 +118,8 @@ inline double of_ints(int hi, int lo) { const uint64_t u = (uint64_t)(uint32_t)h
 #define __shfl_up(v, d, w) emu::from_lane((v), emu::lane() >= (d) ? emu::lane() - (d) : emu::lane())
 #define __ffsll(x) __builtin_ffsll((long long)(x))
 #define __clzll(x) __builtin_clzll((unsigned long long)(x))
+#define __builtin_amdgcn_readfirstlane(x) (x)
+#define __builtin_amdgcn_readlane(v, l) emu::from_lane((v), (l))
 #define __ballot(p) emu::ballot(p)
 #define __double2loint(d) emu::lo_int(d)
 #define __double2hiint(d) emu::hi_int(d)

@@ -199,6 +199,24 @@ def test_null_structs_and_size_queries():
     assert hipdec.verify_drafts_workspace(2, 3, 32768) >= 2 * 4 * 8 * 16
 
 
+def test_a_workspace_serves_every_smaller_call():
+    rng = np.random.default_rng(1)
+    for _ in range(60):
+        kvh, g = int(rng.choice([1, 2, 3, 8, 12, 32])), int(rng.choice([1, 2, 4, 7, 18]))
+        n, length = int(rng.integers(1, 80)), int(2 ** rng.uniform(0, 17))
+        c = cache(kv_heads=kvh, hd=64, stride_page=16 * kvh * 64, stride_slot=kvh * 64, stride_head=64)
+        size = hipdec.attention_paged_workspace(n, kvh * g, kvh, 64, length)
+        for _ in range(20):
+            # (the workspace is looked at before the pointers, which are no device memory)
+            refused(lambda: attention(cache=c, n_rows=int(rng.integers(1, n + 1)), heads=kvh * g, max_len=int(rng.integers(0, length + 1)),
+                                      workspace=FAKE if size else None, workspace_bytes=size), "device")
+        s, k, v = int(rng.integers(1, 70)), int(rng.integers(0, 9)), int(2 ** rng.uniform(0, 18))
+        size = hipdec.verify_drafts_workspace(s, k, v)
+        for _ in range(20):
+            refused(lambda: verify(n_seqs=int(rng.integers(1, s + 1)), max_drafts=int(rng.integers(0, k + 1)), vocab=int(rng.integers(1, v + 1)),
+                                   workspace_bytes=size), "device")
+
+
 def test_errors_are_each_thread_s_own():
     import threading
     refused(lambda: attention(scale=0.0), "scale")
