@@ -308,7 +308,8 @@ int hipdec_sample_fullvocab_noalloc(const float *d_logits, size_t vocab, const f
  * No counterpart in the reference, whose cache is one contiguous window per model and which decodes one
  * token at a time.  They are for programs that keep requests of their own: every d_ pointer is DEVICE
  * memory of the current device, the kernels are enqueued on `stream` (a hipStream_t of the current device,
- * NULL = its default stream) without waiting for them, nothing is allocated and nothing is kept between
+ * NULL = its default stream, which hipStreamLegacy names too; hipStreamPerThread is taken as the current
+ * device's) without waiting for them, nothing is allocated and nothing is kept between
  * calls, so a call can be recorded into a graph.  Workspaces are the caller's: one per call in flight (two
  * streams, or two graphs that may run at once, need one each).  Structs are read before the call returns.
  * Errors are reported through hipdec_last_error(NULL) on the calling thread; after a refusal

@@ -22,6 +22,8 @@ int launched(const char *entry, hipError_t e) {
     (void)hipGetLastError();
     return hipdec_op_error(HIPDEC_ERR_HIP, entry, hipGetErrorString(e));
 }
+// The caller's stream; the handle that names the default one is that.
+hipStream_t stream_of(void *stream) { return stream == (void *)hipStreamLegacy ? nullptr : (hipStream_t)stream; }
 // A launch with its own error, not whatever an earlier call of the program has left behind.
 template <typename A> hipError_t start(void (*kernel)(A), uint64_t grid, int threads, hipStream_t s, const A &a) {
     void *args[] = {(void *)&a};
@@ -38,7 +40,7 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 const char *wrong_place(std::initializer_list<const void *> buffers, void *stream) {
     int dev = -1;
     if (hipGetDevice(&dev) != hipSuccess) { (void)hipGetLastError(); return "no current device"; }
-    if (stream) {
+    if (stream && stream != (void *)hipStreamPerThread) {    // (that one is the current device's, and no object to be asked)
         hipDevice_t of = -1;
         if (hipStreamGetDevice((hipStream_t)stream, &of) != hipSuccess) { (void)hipGetLastError(); return "not a stream"; }
         if ((int)of != dev) return "the stream is of another device than the current one";
@@ -195,7 +197,7 @@ int hipdec_rope_append_paged(const hipdec_rope *rope, const hipdec_paged_cache *
         return refuse(me, "rows overlap: a stride is smaller than its row");
     if (rows->d_q == rows->d_q_out && rows->q_stride != rows->q_out_stride) return refuse(me, "in place, both strides must be equal");
     if ((bad = wrong_place({rows->d_q, rows->d_k, rows->d_v, rows->d_q_out, rows->d_positions, rows->d_slots, rows->d_seqs, rope->d_freq,
-                            cache->k, cache->v, cache->page_table}, stream)))
+                            cache->k, cache->v, cache->page_table}, stream_of(stream))))
         return refuse(me, bad);
 
     RopeArgs a{view(*cache), rows->d_q, rows->d_k, rows->d_v, rows->d_q_out, rows->q_stride, rows->k_stride, rows->v_stride,
@@ -212,7 +214,7 @@ int hipdec_rope_append_paged(const hipdec_rope *rope, const hipdec_paged_cache *
     const uint64_t grid = rows->n_rows * a.parts;
     if (!grid_fits(grid, ROPE_THREADS)) return refuse(me, "n_rows out of range");
     const bool rb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;
-    hipStream_t s = (hipStream_t)stream;
+    hipStream_t s = stream_of(stream);
     if (rb) return launched(me, cb ? go_rope<true, true>(a, wide, grid, s) : go_rope<true, false>(a, wide, grid, s));
     return launched(me, cb ? go_rope<false, true>(a, wide, grid, s) : go_rope<false, false>(a, wide, grid, s));
 }
@@ -253,7 +255,7 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
     if (need && (!d_workspace || workspace_bytes < need || !aligned16(d_workspace)))
         return refuse(me, "workspace missing, too small (hipdec_attention_paged_workspace) or not 16-byte aligned");
     if ((bad = wrong_place({rows->d_q, rows->d_out, rows->d_lens, rows->d_seqs, cache->k, cache->v, cache->page_table,
-                            need ? d_workspace : nullptr}, stream)))
+                            need ? d_workspace : nullptr}, stream_of(stream))))
         return refuse(me, bad);
 
     const int g = (int)(rows->heads / cache->kv_heads), tiles = (g + 15) / 16;
@@ -264,7 +266,7 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
                 g, tiles, (int)(rows->max_len < slots ? rows->max_len : slots), p.chunk, p.splits,
                 rows->scale * 1.44269504088896340736f, po, po + rows->n_rows * rows->heads * p.splits * cache->hd};
     const bool qb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;
-    hipStream_t s = (hipStream_t)stream;
+    hipStream_t s = stream_of(stream);
     switch (cache->hd) {
     case 64: return launched(me, go_attention<64>(qb, cb, a, grid, joins, s));
     case 128: return launched(me, go_attention<128>(qb, cb, a, grid, joins, s));
@@ -304,7 +306,7 @@ int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t wor
         return refuse(me, "workspace missing, too small (hipdec_verify_drafts_workspace) or not 16-byte aligned");
     if (!grid_fits(rows * c.n, VF_STATS)) return refuse(me, "n_seqs * max_drafts * vocab out of range");
     if ((bad = wrong_place({d->d_logits, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms, d->d_tokens, d->d_accepted,
-                            d_workspace}, stream)))
+                            d_workspace}, stream_of(stream))))
         return refuse(me, bad);
     VfStat *st = (VfStat *)d_workspace;
     VfPlace *places = (VfPlace *)(st + rows * c.n);
@@ -312,7 +314,7 @@ int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t wor
     const VerifyArgs a{d->d_logits, d->row_stride, d->prob_stride, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms,
                        (int)d->n_seqs, (int)d->max_drafts, (int)d->vocab, c.n, greedy ? 0.0 : log2e / (double)d->temperature,
                        cap, cap > 0.0 ? 2.0 * log2e / cap : 0.0, st, (double *)(places + d->n_seqs), places, d->d_tokens, d->d_accepted};
-    hipStream_t s = (hipStream_t)stream;
+    hipStream_t s = stream_of(stream);
     return launched(me, d->dtype == HIPDEC_ROWS_BF16 ? go_verify<true>(a, c.per, s) : go_verify<false>(a, c.per, s));
 }
 

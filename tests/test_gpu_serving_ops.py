@@ -607,6 +607,18 @@ def test_two_streams_at_once_with_workspaces_of_their_own(hip):
         hip.ok(hip.rt.hipStreamDestroy(s))
 
 
+@pytest.mark.parametrize("handle", [None, 1, 2])             # the default stream, its other handle, the thread's own
+def test_the_streams_that_are_no_objects(hip, handle):
+    rng = np.random.default_rng(41)
+    lens = [40, 700]
+    cache = Cache(hip, rng, lens, 16, 2, 64, True, False)
+    check_attention(hip, cache, Rows(rng.standard_normal((2, 4, 64)).astype(np.float32), True), None, lens, stream=handle)
+    case = draft_case(rng, 2, 3, 900, False, 0.9, True)
+    tokens, accepted = verify(hip, *case[:4], 0.9, 0.0, case[4], stream=handle)
+    want, want_acc = verified(case[0].x, *case[1:4], 0.9, 0.0, case[4])
+    assert np.array_equal(accepted, want_acc) and np.array_equal(tokens, want)
+
+
 def test_repeated_calls_give_the_same_bits(hip):
     rng = np.random.default_rng(31)
     lens = [5000, 64, 1999, 2000]
