@@ -144,12 +144,12 @@ template <bool RB, bool CB, int NP> __global__ __launch_bounds__(ROPE_THREADS) v
 // precision beyond its own.  The fp32 instruction has room: 64 cached numbers per 32 clocks and SIMD are 32 bytes a
 // clock and CU of a bf16 cache, three times what HBM delivers.  FEW: up to four heads per key head use the 4 x 4 form
 // (16 independent blocks: four heads, the values of four dim groups and one of four keys), 64 numbers in 8 clocks; the
-// columns of the score tile then repeat every four, and the four lane groups keep sums over keys of their own.
-// (eight requests of 12 single heads 19.9 -> 17.2 us.)
+// columns of the score tile then repeat every four, and the four lane groups keep sums over keys of their own (64 ragged
+// requests 220 -> 212 us together with the smaller blocks below).
 //   K of a bf16 cache goes into the bf16 instruction as it is; fp32 queries are three bf16 numbers each (24 bits),
 //   bf16 queries are one.  K of an fp32 cache uses the fp32 instruction.
-// Measured (MI355X, listed sizes): 64 requests of 1 .. 8192 slots, 32 heads over 8, bf16 (1.09 GB): 212 us, 5.2 TB/s; one
-// request of 65536: 54.7 us, 4.9 TB/s; 64 x 4096 evenly 5.5 TB/s; a large copy reaches 4.7.
+// Measured (MI355X, listed sizes): 64 requests of 1 .. 8192 slots, 32 heads over 8, bf16 (1.09 GB): 211 us, 5.2 TB/s; one
+// request of 65536: 54.4 us, 4.9 TB/s; 64 x 4096 evenly 5.5 TB/s; a large copy reaches 4.7.
 struct PagedAttn {
     PagedView c;
     const void *q;
@@ -214,7 +214,7 @@ template <int HD, bool QB, bool CB, bool FEW, int WAVES> __global__ __launch_bou
     const int split = blockIdx.x / per, rest = blockIdx.x % per;
     const int units = a.c.kv_heads * a.tiles, row = rest / units, unit = rest % units;
     const int kvh = unit / a.tiles, g0 = (unit % a.tiles) * 16, gn = min(16, a.g - g0), head0 = kvh * a.g + g0;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), col = lane & 15, grp = lane >> 4;
     const int qcol = FEW ? col & 3 : col;                    // the query head that column `col` is
     int seq;
     const int len = pg_len(a, row, seq);
