@@ -14,7 +14,7 @@
 // probabilities 17.5 us; 64 of up to 5 over 131071 bf16 logits with a soft cap 82 us, where a vector instruction issues in
 // 98 % of the statistics' cycles (60 per logit, 44 of them 64 bits wide; 27 without a cap).
 #pragma once
-#include "hipdec_common.h"
+#include "hipdec_wave64.h"
 
 // A chunk is what one wave takes: 64 * PER logits.  No barrier stands between a chunk's loads and its result, so the waves of
 // a CU drift apart and one's loads run under another's arithmetic (with a workgroup to a chunk and two barriers in it
