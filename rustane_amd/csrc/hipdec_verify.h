@@ -94,39 +94,48 @@ template <int PER, bool NEAR> __device__ __forceinline__ void vf_guess(const Ver
 // this thread's wave, known to be one number for the whole wave
 __device__ __forceinline__ int vf_wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
-// 2^y for -1021 <= y <= 1022: y = n + f with |f| <= 1/2, the series of 2^f = e^(f ln 2) up to its 11th power (the rest
-// is below 0.3466^12 / 12! = 7e-15 of it), scaled by 2^n in the exponent's bits.  n is read off the last bits of
-// y + 1.5 * 2^52.  The kernels' time on large calls is their instructions, most of them these 19 for each logit.
-__device__ __forceinline__ double vf_exp2(double y) {
-    const double whole = 6755399441055744.0, t = y + whole, f = y - (t - whole);
-    double p = 4.4455382718708116e-10;                       // (ln 2)^k / k!, k = 11 .. 0
-    p = fma(p, f, 7.054911620801123e-09);
-    p = fma(p, f, 1.01780860092397e-07);
-    p = fma(p, f, 1.321548679014431e-06);
-    p = fma(p, f, 1.5252733804059841e-05);
-    p = fma(p, f, 1.540353039338161e-04);
-    p = fma(p, f, 1.3333558146428443e-03);
-    p = fma(p, f, 9.618129107628477e-03);
-    p = fma(p, f, 5.550410866482158e-02);
-    p = fma(p, f, 2.4022650695910072e-01);
-    p = fma(p, f, 6.931471805599453e-01);
-    p = fma(p, f, 1.0);
-    return __hiloint2double(__double2hiint(p) + (int)((unsigned)__double2loint(t) << 20), __double2loint(p));
+// 2^y = 2^n 2^f for -1021 <= y <= 1022 with n = y to the nearest, read off the last bits of y + 1.5 * 2^52; f = y - n.
+__device__ __forceinline__ double vf_parts(double y, uint32_t &n) {
+    const double whole = 6755399441055744.0, t = y + whole;
+    n = (uint32_t)__double2loint(t);
+    return y - (t - whole);
 }
-// softcap(x) = cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1): off by 1e-15 of the cap, absolutely, which is what
-// the exponent behind it needs
+// (2^f - 1) / f for |f| <= 1/2: the polynomial of degree 8 whose product with f comes nearest to 2^f - 1, relative to 2^f
+// (least squares in extended precision, reweighted until the extremes were level): 1.5e-14 of 2^f, 2^0 exactly 1.
+// (The series needs two more terms for 7e-15.)  The kernels' time on large calls is their instructions, most of them these.
+__device__ __forceinline__ double vf_slope(double f) {
+    double p = 1.0148339389471021e-07;
+    p = fma(p, f, 1.3258335516349176e-06);
+    p = fma(p, f, 1.5252990022790325e-05);
+    p = fma(p, f, 1.5403440883887646e-04);
+    p = fma(p, f, 1.333355762545611e-03);
+    p = fma(p, f, 9.61812918116482e-03);
+    p = fma(p, f, 5.550410866841585e-02);
+    p = fma(p, f, 2.4022650695722814e-01);
+    return fma(p, f, 6.931471805598851e-01);
+}
+__device__ __forceinline__ double vf_exp2(double y) {
+    uint32_t n;
+    const double f = vf_parts(y, n), p = fma(vf_slope(f), f, 1.0);
+    return __hiloint2double(__double2hiint(p) + (int)(n << 20), __double2loint(p));
+}
+// softcap(x) / cap = tanh(x / cap) = E / (E + 2) with E = e^(2 x / cap) - 1 = 2^n (2^f - 1) + (2^n - 1): nothing cancels, so
+// it is right to 2e-14 of itself, at a cap far above the logits too.  Past 2^+-100 it is +-1.  (The plain form without cap.)
 template <bool CAP> __device__ __forceinline__ double vf_capped(const VerifyArgs &a, float x) {
     if (!CAP) return (double)x;
-    const double d = vf_exp2(fmin(fmax((double)x * a.cap_k, -1000.0), 1000.0)) + 1.0;
-    double r = __builtin_amdgcn_rcp(d);                      // 1 / d by Newton's method: each step squares the error
+    const float far = 34.657359f * (float)a.cap;             // 100 of 2 log2(e) / cap
+    uint32_t n;
+    const double f = vf_parts((double)fminf(fmaxf(x, -far), far) * a.cap_k, n);
+    const double two_n = __hiloint2double((int)(0x3ff00000u + (n << 20)), 0);
+    const double e = fma(vf_slope(f) * f, two_n, two_n - 1.0), d = e + 2.0;
+    double r = __builtin_amdgcn_rcp(d);                      // good to 2^-24; Newton's step squares that
     r = fma(r, fma(-d, r, 1.0), r);
-    r = fma(r, fma(-d, r, 1.0), r);
-    return fma(-2.0 * a.cap, r, a.cap);
+    return e * r;
 }
-// exp((z - max z) / T) with ztop = the row's maximum z; impossible tokens, and what lies 2^1021 below the maximum, are 0.
+// exp((z - max z) / T) with ztop = the row's maximum, as vf_capped has it; impossible tokens, and what lies 2^1021 below the maximum, are 0.
 // EXACT_ZERO: whether the difference of 0 and 2^-1021 counts (it does where a token is picked, not in a row's sum).
 template <bool CAP, bool EXACT_ZERO> __device__ __forceinline__ double vf_weight(const VerifyArgs &a, float x, double ztop) {
-    const double y = fmax((vf_capped<CAP>(a, x) - ztop) * a.k, -1021.0);   // (a row of nothing else: -inf + inf, a NaN, counts as -1021)
+    const double y = fmax((vf_capped<CAP>(a, x) - ztop) * (CAP ? a.cap * a.k : a.k), -1021.0);   // (a row of nothing else: -inf + inf, a NaN, counts as -1021)
     const double w = vf_exp2(y);
     if (CAP) return x == -INFINITY ? 0.0 : w;
     return EXACT_ZERO ? y > -1021.0 ? w : 0.0 : w;

@@ -607,6 +607,16 @@ def test_two_streams_at_once_with_workspaces_of_their_own(hip):
         hip.ok(hip.rt.hipStreamDestroy(s))
 
 
+@pytest.mark.parametrize("cap", [1e8, 1e14, 1e30, 3.4e38])
+def test_a_cap_far_above_the_logits_changes_nothing(hip, cap):
+    """|softcap(x) - x| < |x|^3 / (3 cap^2): below 2e-12 for |x| <= 40, as small as the draws' own rounding."""
+    rng = np.random.default_rng(43)
+    case = draft_case(rng, 6, 4, 2000, False, 0.8, True)
+    plain, plain_acc = verify(hip, *case[:4], 0.8, 0.0, case[4])
+    tokens, accepted = verify(hip, *case[:4], 0.8, cap, case[4])
+    assert np.array_equal(accepted, plain_acc) and np.array_equal(tokens, plain)
+
+
 @pytest.mark.parametrize("handle", [None, 1, 2])             # the default stream, its other handle, the thread's own
 def test_the_streams_that_are_no_objects(hip, handle):
     rng = np.random.default_rng(41)
