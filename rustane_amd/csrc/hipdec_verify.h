@@ -78,13 +78,16 @@ template <bool B16, int PER, bool NEAR> __device__ __forceinline__ void vf_logit
         for (int i = 0; i < PER; ++i) x[i] = mine + i * step < a.vocab ? vf_number<B16>(raw[i]) : -INFINITY;
     }
 }
+// a probability of the draft's, or a random number, as it counts: a negative one is 0 (a token that the target cannot give, or that
+// lies behind the vocabulary, would have a rest otherwise, and a draft that it cannot give would be kept); a NaN stays one
+__device__ __forceinline__ float vf_from0(float x) { return x < 0.0f ? 0.0f : x; }
 // the draft's probabilities of the same tokens
 template <int PER, bool NEAR> __device__ __forceinline__ void vf_guess(const VerifyArgs &a, long long draft, int chunk, float *q) {
     const int lane = threadIdx.x & 63, step = NEAR ? 1 : WAVE, mine = chunk * PER * WAVE + (NEAR ? lane * PER : lane);
     if (a.probs) {
         const float *p = a.probs + draft * a.prob_stride;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) q[i] = p[min(mine + i * step, a.vocab - 1)];   // (behind the vocabulary the target has nothing)
+        for (int i = 0; i < PER; ++i) q[i] = vf_from0(p[min(mine + i * step, a.vocab - 1)]);   // (behind the vocabulary the target has nothing)
     } else {
         const int d = a.drafts[draft];
 #pragma unroll
@@ -203,8 +206,8 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(VF_DECIDE) v
         const int at = real ? d : 0;
         const float logit = vf_logit<B16>(a, row, at), x = real ? logit : -INFINITY;
         const bool sampled = a.k > 0.0 && i < n;
-        const double q = sampled && a.probs ? (double)a.probs[((long long)s * K + i) * a.prob_stride + at] : 1.0;
-        const double u = sampled ? (double)a.u[(size_t)s * (K + 1) + i] : 0.0;
+        const double q = sampled && a.probs ? (double)vf_from0(a.probs[((long long)s * K + i) * a.prob_stride + at]) : 1.0;
+        const double u = sampled ? (double)vf_from0(a.u[(size_t)s * (K + 1) + i]) : 0.0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) if (lane + 64 * j >= a.chunks) mine[j] = VfStat{0.0, -INFINITY, 0xffffffffu};
 #pragma unroll
@@ -258,7 +261,7 @@ template <bool B16, bool CAP, int PER> __global__ __launch_bounds__(WAVE) void k
     const int s = blockIdx.x, lane = threadIdx.x, K = a.max_drafts;
     const int n = vf_drafts(a, s);
     const VfPlace at = a.places[s];
-    const float u = a.u[(size_t)s * (K + 1) + K];
+    const float u = vf_from0(a.u[(size_t)s * (K + 1) + K]);
     double mine[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) mine[j] = a.sums[(size_t)s * a.chunks + min(4 * lane + j, a.chunks - 1)];
