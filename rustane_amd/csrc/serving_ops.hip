@@ -30,7 +30,7 @@ template <typename A> hipError_t start(void (*kernel)(A), uint64_t grid, int thr
     return hipLaunchKernel((const void *)kernel, dim3((unsigned)grid), dim3((unsigned)threads), args, 0, s);
 }
 
-// (a grid's threads are counted in 32 bits)
+// (a grid's threads are counted in 32 bits; every launch of a call is looked at before its first)
 bool grid_fits(uint64_t groups, uint64_t threads) { return groups <= 0x7fffffffu && groups * threads <= 0xffffffffu; }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -104,9 +104,10 @@ uint64_t attention_bytes(uint64_t n_rows, uint32_t heads, uint32_t kv_heads, uin
     return most * heads * (hd + 2) * sizeof(float);
 }
 
+// Waves of a workgroup where one split writes the result (eight of the widest fp32 heads would not keep their registers).
+constexpr int wide_waves(uint32_t hd, bool cb) { return hd * (cb ? 2 : 4) <= 512 ? 8 : 4; }
 template <int HD, bool QB, bool CB, bool FEW> hipError_t go_attention(const PagedAttn &a, uint64_t grid, uint64_t joins, hipStream_t s) {
-    // (eight waves of the widest fp32 heads would not keep their registers)
-    constexpr int WIDE = HD * (CB ? 2 : 4) <= 512 ? 8 : 4;
+    constexpr int WIDE = wide_waves(HD, CB);
     if (a.splits == 1) return start(k_attn_paged<HD, QB, CB, FEW, WIDE>, grid, 64 * WIDE, s, a);
     const hipError_t e = start(k_attn_paged<HD, QB, CB, FEW, 4>, grid, 256, s, a);
     return e != hipSuccess ? e : start(k_attn_paged_join<HD, QB>, joins, 256, s, a);
@@ -137,11 +138,18 @@ uint64_t verify_bytes(uint64_t n_seqs, uint32_t max_drafts, int chunks) {
     return n_seqs * ((max_drafts + 1) * chunks * sizeof(VfStat) + chunks * sizeof(double) + sizeof(VfPlace));
 }
 
+// Workgroups of the statistics and of the decision.
+struct VerifyGrids { uint64_t stats, decide; };
+VerifyGrids verify_grids(uint64_t n_seqs, uint32_t max_drafts, int chunks, bool greedy) {
+    const int few = (chunks + VF_STATS / WAVE - 1) / (VF_STATS / WAVE), more = (chunks + VF_DECIDE / WAVE - 1) / (VF_DECIDE / WAVE);
+    return VerifyGrids{n_seqs * (max_drafts + 1) * few, greedy ? n_seqs : n_seqs * more};
+}
+
 template <bool B16, bool CAP, int PER> hipError_t go_verify(const VerifyArgs &a, hipStream_t s) {
-    const uint64_t seqs = a.n_seqs, few = (a.chunks + VF_STATS / WAVE - 1) / (VF_STATS / WAVE), more = (a.chunks + VF_DECIDE / WAVE - 1) / (VF_DECIDE / WAVE);
-    hipError_t e = start(k_verify_stats<B16, CAP, PER>, seqs * (a.max_drafts + 1) * few, VF_STATS, s, a);
-    if (e == hipSuccess) e = start(k_verify_decide<B16, CAP, PER>, a.k > 0.0 ? seqs * more : seqs, VF_DECIDE, s, a);
-    if (e == hipSuccess && a.k > 0.0) e = start(k_verify_draw<B16, CAP, PER>, seqs, WAVE, s, a);
+    const VerifyGrids g = verify_grids(a.n_seqs, a.max_drafts, a.chunks, !(a.k > 0.0));
+    hipError_t e = start(k_verify_stats<B16, CAP, PER>, g.stats, VF_STATS, s, a);
+    if (e == hipSuccess) e = start(k_verify_decide<B16, CAP, PER>, g.decide, VF_DECIDE, s, a);
+    if (e == hipSuccess && a.k > 0.0) e = start(k_verify_draw<B16, CAP, PER>, (uint64_t)a.n_seqs, WAVE, s, a);
     return e;
 }
 template <bool B16> hipError_t go_verify(const VerifyArgs &a, int per, hipStream_t s) {
@@ -250,7 +258,12 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
         return refuse(me, "queries, outputs and the cache must be 16-byte aligned, with strides of whole 16 bytes");
 
     const uint64_t slots = (uint64_t)cache->max_pages * cache->page_size;
-    const Split p = split_of(rows->n_rows, cache->kv_heads, rows->heads / cache->kv_heads, rows->max_len);
+    const bool qb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;
+    const int g = (int)(rows->heads / cache->kv_heads), tiles = (g + 15) / 16;
+    const Split p = split_of(rows->n_rows, cache->kv_heads, (uint32_t)g, rows->max_len);
+    const uint64_t grid = rows->n_rows * cache->kv_heads * tiles * p.splits, joins = rows->n_rows * rows->heads;
+    if (!grid_fits(grid, p.splits == 1 ? 64 * wide_waves(cache->hd, cb) : 256) || (p.splits > 1 && !grid_fits(joins, 256)))
+        return refuse(me, "n_rows * heads * max_len out of range");
     const uint64_t need = p.splits == 1 ? 0 : rows->n_rows * rows->heads * p.splits * (cache->hd + 2) * sizeof(float);
     if (need && (!d_workspace || workspace_bytes < need || !aligned16(d_workspace)))
         return refuse(me, "workspace missing, too small (hipdec_attention_paged_workspace) or not 16-byte aligned");
@@ -258,14 +271,10 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
                             need ? d_workspace : nullptr}, stream_of(stream))))
         return refuse(me, bad);
 
-    const int g = (int)(rows->heads / cache->kv_heads), tiles = (g + 15) / 16;
-    const uint64_t grid = rows->n_rows * cache->kv_heads * tiles * p.splits, joins = rows->n_rows * rows->heads;
-    if (!grid_fits(grid, 512) || !grid_fits(joins, 256)) return refuse(me, "n_rows * heads * max_len out of range");
     float *po = (float *)d_workspace;
     PagedAttn a{view(*cache), rows->d_q, rows->d_out, rows->q_stride, rows->out_stride, rows->d_lens, rows->d_seqs, (int)rows->heads,
                 g, tiles, (int)(rows->max_len < slots ? rows->max_len : slots), p.chunk, p.splits,
                 rows->scale * 1.44269504088896340736f, po, po + rows->n_rows * rows->heads * p.splits * cache->hd};
-    const bool qb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;
     hipStream_t s = stream_of(stream);
     switch (cache->hd) {
     case 64: return launched(me, go_attention<64>(qb, cb, a, grid, joins, s));
@@ -301,10 +310,11 @@ int hipdec_verify_drafts(const hipdec_drafts *d, void *d_workspace, uint64_t wor
         return refuse(me, "rows overlap: a stride is smaller than the vocabulary");
     const uint64_t rows = d->n_seqs * (d->max_drafts + 1);
     const Chunks c = chunks_of(rows, d->vocab);
+    const VerifyGrids g = verify_grids(d->n_seqs, d->max_drafts, c.n, greedy);   // (the draw's are fewer than either)
+    if (!grid_fits(g.stats, VF_STATS) || !grid_fits(g.decide, VF_DECIDE)) return refuse(me, "n_seqs * max_drafts * vocab out of range");
     const uint64_t need = verify_bytes(d->n_seqs, d->max_drafts, c.n);
     if (!d_workspace || workspace_bytes < need || !aligned16(d_workspace))
         return refuse(me, "workspace missing, too small (hipdec_verify_drafts_workspace) or not 16-byte aligned");
-    if (!grid_fits(rows * c.n, VF_STATS)) return refuse(me, "n_seqs * max_drafts * vocab out of range");
     if ((bad = wrong_place({d->d_logits, d->d_drafts, d->d_n_drafts, d->d_draft_probs, d->d_uniforms, d->d_tokens, d->d_accepted,
                             d_workspace}, stream_of(stream))))
         return refuse(me, bad);

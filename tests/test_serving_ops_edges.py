@@ -6,7 +6,9 @@ import subprocess
 
 import pytest
 
+from rustane_amd.hipdec import KvDtype, PagedCache, RowDtype
 from test_kernel_emulation import EMU, ROOT, host_clang
+from test_serving_ops import FAKE, attention, refused, verify
 
 
 @pytest.fixture(scope="module")
@@ -36,3 +38,35 @@ def emulated(tmp_path_factory):
 # ---------------------------------------------------------------- verification of drafts
 def test_negative_probabilities_and_random_numbers_count_as_zero(emulated):
     emulated("verify_edges", "negative_numbers")
+
+
+# ---------------------------------------------------------------- sizes at the launches' limits (no GPU: the host decides)
+HUGE = 1 << 62                # workspace bytes
+
+
+@pytest.mark.parametrize("kw,text", [
+    # a launch counts its threads in 32 bits, and every launch of a call is looked at before the first
+    (dict(n_seqs=9_000_000, max_drafts=0, vocab=256), "out of range"),       # the decision's workgroups of 512
+    (dict(n_seqs=8_388_607, max_drafts=0, vocab=256), "device"),
+    (dict(n_seqs=9_000_000, max_drafts=0, vocab=256, temperature=0.0), "out of range"),
+    (dict(n_seqs=(1 << 24) - 1, max_drafts=1, vocab=1024), "out of range"),  # the statistics' of 256
+    (dict(n_seqs=1 << 17, max_drafts=0, vocab=131071, dtype=RowDtype.BF16), "device"),   # 2^17 rows of 128 chunks, four to a workgroup
+    (dict(n_seqs=1 << 19, max_drafts=0, vocab=131071, dtype=RowDtype.BF16), "out of range"),
+])
+def test_verification_counts_its_launches_as_they_are(kw, text):
+    refused(lambda: verify(workspace_bytes=HUGE, **kw), text)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(n_rows=8192, heads=32, max_len=131072), "device"),                 # 8192 x 8 x 128 workgroups of 256
+    (dict(n_rows=16384, heads=32, max_len=131072), "out of range"),
+    (dict(n_rows=1 << 20, heads=8, max_len=250), "out of range"),            # one launch: 2^20 x 8 workgroups of 512 are one too many,
+    (dict(n_rows=(1 << 20) - 1, heads=8, max_len=250), "device"),
+    (dict(n_rows=1 << 20, heads=8, max_len=250, hd=256, kv_dtype=KvDtype.F32), "device"),    # ... of 256 are not
+    (dict(n_rows=1 << 24, heads=8, max_len=1), "out of range"),
+])
+def test_attention_counts_its_launches_as_they_are(kw, text):
+    kw = dict(kw)
+    hd, dt = kw.pop("hd", 128), kw.pop("kv_dtype", KvDtype.BF16)
+    c = PagedCache.make(FAKE, FAKE, dt, n_pages=4, page_size=16, kv_heads=8, hd=hd, page_table=FAKE, n_seqs=2, max_pages=2)
+    refused(lambda: attention(cache=c, workspace=FAKE, workspace_bytes=HUGE, **kw), text)
