@@ -138,7 +138,9 @@ template <bool CAP> __device__ __forceinline__ double vf_capped(const VerifyArgs
 // exp((z - max z) / T) with ztop = the row's maximum, as vf_capped has it; impossible tokens, and what lies 2^1021 below the maximum, are 0.
 // EXACT_ZERO: whether the difference of 0 and 2^-1021 counts (it does where a token is picked, not in a row's sum).
 template <bool CAP, bool EXACT_ZERO> __device__ __forceinline__ double vf_weight(const VerifyArgs &a, float x, double ztop) {
-    const double y = fmax((vf_capped<CAP>(a, x) - ztop) * (CAP ? a.cap * a.k : a.k), -1021.0);   // (a row of nothing else: -inf + inf, a NaN, counts as -1021)
+    double y = fmax((vf_capped<CAP>(a, x) - ztop) * (CAP ? a.cap * a.k : a.k), -1021.0);   // (a row of nothing else: -inf + inf, a NaN, counts as -1021)
+    // (the cap's last bits can put a logit that it saturates above the maximum's, which a small temperature multiplies without limit)
+    if (CAP) y = fmin(y, 0.0);
     const double w = vf_exp2(y);
     if (CAP) return x == -INFINITY ? 0.0 : w;
     return EXACT_ZERO ? y > -1021.0 ? w : 0.0 : w;

@@ -1,5 +1,5 @@
 // More of the draft-verification kernels' own source on the CPU, one check per name on the command line, against a restatement
-// in long double: numbers outside their range.  Unlike verify_drafts.cpp it runs the waves' running sums and maxima from their
+// in long double: numbers outside their range, temperatures near 0.  Unlike verify_drafts.cpp it runs the waves' running sums and maxima from their
 // own source too (kernel_wave64.inc: the data-parallel moves are stood in for, not the functions above them), and the
 // reciprocal is good to 24 bits only, as the instruction is.
 #define wave_scan_f64 whole_scan_f64
@@ -159,8 +159,32 @@ static int negative_numbers() {
     return wrong;
 }
 
+// A soft cap that every other logit saturates, at temperatures down to the smallest: the saturated ones lie within the last bits of
+// each other, and nothing but one of them may be kept or drawn.
+static int tiny_temperatures() {
+    int wrong = 0;
+    for (float T : {1e-12f, 1e-18f, 1e-20f, 1e-30f, 1.17549435e-38f})
+        for (bool with_probs : {false, true}) {
+            Drafts c(8, 3, 700, T, 2.0f, with_probs);
+            for (int s = 0; s < c.S; ++s)
+                for (int i = 0; i <= c.K; ++i) {
+                    for (int j = 0; j < c.V; ++j) c.row(s, i)[j] = j % 2 ? 40.0f + 30.0f * uniform() : normal(2.0f);
+                    for (int j = 0; i < c.K && j < c.V; ++j) c.prob(s, i)[j] = 1.0f / c.V;
+                    if (i < c.K) c.d[s * c.K + i] = (int)(rng() % c.V);
+                }
+            const Decided got = run<true, 4>(c);
+            for (int s = 0; s < c.S; ++s)
+                for (int i = 0; i <= c.K; ++i) {
+                    const uint32_t t = got.tokens[s * (c.K + 1) + i];
+                    const bool ok = i > got.accepted[s] ? t == 0xffffffffu : t < (uint32_t)c.V && t % 2 == 1;
+                    if (!ok) { ++wrong; std::printf("  temperature %g: sequence %d place %d has %u\n", T, s, i, t); }
+                }
+        }
+    return wrong;
+}
+
 int main(int argc, char **argv) {
-    const struct { const char *name; int (*check)(); } checks[] = {{"negative_numbers", negative_numbers}};
+    const struct { const char *name; int (*check)(); } checks[] = {{"negative_numbers", negative_numbers}, {"tiny_temperatures", tiny_temperatures}};
     for (const auto &c : checks)
         if (argc > 1 && !std::strcmp(argv[1], c.name)) {
             const int wrong = c.check();

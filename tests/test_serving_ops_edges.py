@@ -40,6 +40,10 @@ def test_negative_probabilities_and_random_numbers_count_as_zero(emulated):
     emulated("verify_edges", "negative_numbers")
 
 
+def test_tiny_temperatures_with_a_saturated_soft_cap(emulated):
+    emulated("verify_edges", "tiny_temperatures")
+
+
 # ---------------------------------------------------------------- sizes at the launches' limits (no GPU: the host decides)
 HUGE = 1 << 62                # workspace bytes
 
