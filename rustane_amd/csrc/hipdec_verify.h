@@ -103,19 +103,21 @@ __device__ __forceinline__ double vf_parts(double y, uint32_t &n) {
     n = (uint32_t)__double2loint(t);
     return y - (t - whole);
 }
-// (2^f - 1) / f for |f| <= 1/2: the polynomial of degree 8 whose product with f comes nearest to 2^f - 1, relative to 2^f
-// (least squares in extended precision, reweighted until the extremes were level): 1.5e-14 of 2^f, 2^0 exactly 1.
-// (The series needs two more terms for 7e-15.)  The kernels' time on large calls is their instructions, most of them these.
+// (2^f - 1) / f for |f| <= 1/2: the polynomial of degree 9 through its values at the ten Chebyshev nodes (worked out in 60 digits),
+// 1.5e-15 of it, so that 2^f near 1 and the soft cap of small logits are right relative to themselves.  (Degree 8 leaves 9e-14: with
+// it the soft cap was off by 2e-13 of itself, and each of up to 262144 borders of a draw by as much of the whole.  The kernels' time
+// on large calls is their instructions, most of them these.)
 __device__ __forceinline__ double vf_slope(double f) {
-    double p = 1.0148339389471021e-07;
-    p = fma(p, f, 1.3258335516349176e-06);
-    p = fma(p, f, 1.5252990022790325e-05);
-    p = fma(p, f, 1.5403440883887646e-04);
-    p = fma(p, f, 1.333355762545611e-03);
-    p = fma(p, f, 9.61812918116482e-03);
-    p = fma(p, f, 5.550410866841585e-02);
-    p = fma(p, f, 2.4022650695722814e-01);
-    return fma(p, f, 6.931471805598851e-01);
+    double p = 7.070977866508138e-09;
+    p = fma(p, f, 1.0205905413765595e-07);
+    p = fma(p, f, 1.3215451633221434e-06);
+    p = fma(p, f, 1.5252672924850737e-05);
+    p = fma(p, f, 1.5403530424776529e-04);
+    p = fma(p, f, 1.3333558200794592e-03);
+    p = fma(p, f, 9.618129107618665e-03);
+    p = fma(p, f, 5.550410866465167e-02);
+    p = fma(p, f, 2.4022650695910075e-01);
+    return fma(p, f, 6.931471805599462e-01);
 }
 __device__ __forceinline__ double vf_exp2(double y) {
     uint32_t n;
@@ -123,7 +125,7 @@ __device__ __forceinline__ double vf_exp2(double y) {
     return __hiloint2double(__double2hiint(p) + (int)(n << 20), __double2loint(p));
 }
 // softcap(x) / cap = tanh(x / cap) = E / (E + 2) with E = e^(2 x / cap) - 1 = 2^n (2^f - 1) + (2^n - 1): nothing cancels, so
-// it is right to 2e-14 of itself, at a cap far above the logits too.  Past 2^+-100 it is +-1.  (The plain form without cap.)
+// it is right to 1e-14 of itself, at a cap far above the logits too.  Past 2^+-100 it is +-1.  (The plain form without cap.)
 template <bool CAP> __device__ __forceinline__ double vf_capped(const VerifyArgs &a, float x) {
     if (!CAP) return (double)x;
     const float far = 34.657359f * (float)a.cap;             // 100 of 2 log2(e) / cap

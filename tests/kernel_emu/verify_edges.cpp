@@ -183,8 +183,33 @@ static int tiny_temperatures() {
     return wrong;
 }
 
+// The soft cap and the exponential against long double.  Allowed: the polynomial's 1.5e-15, the reciprocal's 2^-48 = 3.6e-15 behind
+// one Newton step and some ten roundings of 1.1e-16: 1e-14 of the value; the exponential, without a reciprocal, 4e-15.
+static int elementary_accuracy() {
+    int wrong = 0;
+    long double worst = 0.0, worst_e = 0.0;
+    VerifyArgs a{};
+    for (float cap : {1e-3f, 0.5f, 2.0f, 5.0f, 30.0f, 50.0f, 1e4f, 1e8f, 1e30f}) {
+        a.cap = cap;
+        a.cap_k = 2 * 1.4426950408889634074 / a.cap;
+        for (int i = 0; i < 20000; ++i) {
+            const float x = (i % 2 ? -1.0f : 1.0f) * cap * (float)std::pow(10.0, -12.0 + 13.6 * i / 20000);
+            const long double want = tanhl((long double)x / cap), got = vf_capped<true>(a, x);
+            worst = std::fmax(worst, std::fabs(got / want - 1.0L));
+        }
+    }
+    for (int i = 0; i <= 40000; ++i) {
+        const double y = i < 20000 ? -1021.0 * i / 20000 : -1.0 * (i - 20000) / 20000;
+        worst_e = std::fmax(worst_e, std::fabs((long double)vf_exp2(y) / exp2l(y) - 1.0L));
+    }
+    std::printf("soft cap off by up to %.2Lg of itself, exponential %.2Lg\n", worst, worst_e);
+    wrong += !(worst <= 1e-14L) + !(worst_e <= 4e-15L) + (vf_exp2(0.0) != 1.0) + (vf_capped<true>(a, 0.0f) != 0.0);
+    return wrong;
+}
+
 int main(int argc, char **argv) {
-    const struct { const char *name; int (*check)(); } checks[] = {{"negative_numbers", negative_numbers}, {"tiny_temperatures", tiny_temperatures}};
+    const struct { const char *name; int (*check)(); } checks[] = {{"negative_numbers", negative_numbers}, {"tiny_temperatures", tiny_temperatures},
+                                                               {"elementary_accuracy", elementary_accuracy}};
     for (const auto &c : checks)
         if (argc > 1 && !std::strcmp(argv[1], c.name)) {
             const int wrong = c.check();

@@ -44,6 +44,10 @@ def test_tiny_temperatures_with_a_saturated_soft_cap(emulated):
     emulated("verify_edges", "tiny_temperatures")
 
 
+def test_soft_cap_and_exponential_are_right_to_64_bits(emulated):
+    emulated("verify_edges", "elementary_accuracy")
+
+
 # ---------------------------------------------------------------- sizes at the launches' limits (no GPU: the host decides)
 HUGE = 1 << 62                # workspace bytes
 
