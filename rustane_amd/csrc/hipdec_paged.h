@@ -24,8 +24,9 @@ __device__ __forceinline__ long long pg_offset(const PagedView &c, int page, int
 // Row t at position m: pair i of the first `rot` elements of every query and key head turns by the angle m * freq[i]
 // (pair = elements (2i, 2i + 1), or (i, i + rot / 2) in the half layout), both results scaled by `magnitude`; the
 // other elements and the values pass through.  Queries go to q_out, keys and values to the row's slot of the cache.
-// The angle is reduced in 64 bits (m * freq to whole turns: a position of a million in fp32 is off by a tenth of a
-// radian), its sine and cosine and the turn are fp32, and each result is rounded once, to its own type.
+// The angle, its sine and cosine and their products with the magnitude are 64 bits wide (a position of a million in fp32
+// is off by a tenth of a radian; an angle reduced in 64 bits and rounded to fp32 by 1.9e-7, more than the turn itself); both
+// are rounded to fp32 once, the turn is fp32, and each result is rounded once, to its own type.
 struct RopeArgs {
     PagedView c;
     const void *q, *k, *v;
@@ -66,15 +67,39 @@ template <bool B16, int N> __device__ __forceinline__ void pg_put_n(void *p, lon
     }
 }
 
+// Sine and cosine of `a`, times `by`, rounded once.  a less whole quarter turns n (pi / 2 in two parts, the products exact) lies within
+// pi / 4 of 0, where the Taylor series end with errors of 9e-12 and 4e-13; n's last two bits say which is which, and the signs.
+__device__ __forceinline__ void pg_sincos(double a, double by, float &sn, float &cs) {
+    const double n = rint(a * 0.63661977236758134);
+    const double r = fma(n, -6.123233995736766e-17, fma(n, -1.5707963267948966, a)), z = r * r;
+    double s = -2.5052108385441720e-08, c = 2.0876756987868099e-09;
+    s = fma(s, z, 2.7557319223985893e-06);
+    s = fma(s, z, -1.9841269841269841e-04);
+    s = fma(s, z, 8.3333333333333333e-03);
+    s = fma(s, z, -1.6666666666666667e-01);
+    s = fma(s * z, r, r);
+    c = fma(c, z, -2.7557319223985888e-07);
+    c = fma(c, z, 2.4801587301587302e-05);
+    c = fma(c, z, -1.3888888888888889e-03);
+    c = fma(c, z, 4.1666666666666664e-02);
+    c = fma(c, z, -0.5);
+    c = fma(c, z, 1.0);
+    const int q = (int)(n - 4.0 * floor(0.25 * n));
+    const double p = q & 1 ? c : s, o = q & 1 ? s : c;
+    sn = (float)((q & 2 ? -p : p) * by);
+    cs = (float)(((q + 1) & 2 ? -o : o) * by);
+}
+
 #define ROPE_THREADS 256
-// One workgroup per row and part of its heads.  A thread keeps one unit (NP pairs) of the head and walks the heads,
-// so that its NP angles are worked out once.  NP = 4 wherever the pieces are 4 aligned elements, else 1.
+// One workgroup per row and part of its heads.  Its angles are worked out once, a thread each, and shared; a thread keeps one
+// unit (NP pairs) of the head and walks the heads.  NP = 4 wherever the pieces are 4 aligned elements, else 1.
 template <bool RB, bool CB, int NP> __global__ __launch_bounds__(ROPE_THREADS) void k_rope_append(RopeArgs a) {
+    __shared__ float s_cs[ROPE_THREADS], s_sn[ROPE_THREADS]; // (rot / 2 <= 256)
     const int units = a.hd / (2 * NP), per_pass = ROPE_THREADS / units;
     const int u = threadIdx.x % units, hg = threadIdx.x / units;
     const int t = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
-    if (hg >= per_pass) return;
     const int m = a.pos[t];
+    if ((int)threadIdx.x < a.rot / 2) pg_sincos((double)m * a.freq[threadIdx.x], (double)a.magnitude, s_sn[threadIdx.x], s_cs[threadIdx.x]);
     const int seq = a.seqs ? a.seqs[t] : t, slot = a.slots ? a.slots[t] : m;
     // a row outside the cache (a padding row: slot < 0; a slot, sequence or page that does not exist) writes nothing
     long long at = -1;
@@ -82,15 +107,13 @@ template <bool RB, bool CB, int NP> __global__ __launch_bounds__(ROPE_THREADS) v
         const int page = pg_page(a.c, seq, slot);
         if (page >= 0) at = pg_offset(a.c, page, slot);
     }
+    __syncthreads();
+    if (hg >= per_pass) return;
     const bool turned = u < a.rot / (2 * NP);
     float cs[NP], sn[NP];
     if (turned) {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const double turns = (double)m * (a.freq[u * NP + i] * 0.15915494309189533577);
-            sincospif(2.0f * (float)(turns - rint(turns)), &sn[i], &cs[i]);
-            cs[i] *= a.magnitude; sn[i] *= a.magnitude;
-        }
+        for (int i = 0; i < NP; ++i) { cs[i] = s_cs[u * NP + i]; sn[i] = s_sn[u * NP + i]; }
     }
     const bool half = turned && !a.interleaved;
     const int o0 = half ? NP * u : 2 * NP * u, o1 = half ? a.rot / 2 + NP * u : 2 * NP * u + NP;

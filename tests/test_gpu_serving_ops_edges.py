@@ -1,0 +1,42 @@
+"""Calls of the operators on the caller's device buffers at the edge of what include/hip_decode.h allows, on the GPU, against plain
+fp64 restatements (those of test_gpu_serving_ops.py, whose head derives the tolerances of attention)."""
+import numpy as np
+import pytest
+
+from rustane_amd import hipdec
+from rustane_amd.hipdec import Rope, RopeScaling
+from test_gpu_serving_ops import EPS, Cache, fetch, hip, turned  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- rotary positions
+@pytest.mark.parametrize("hd,rot,interleaved,rows", [(128, 128, True, 3), (64, 64, False, 70), (64, 62, False, 9), (256, 128, True, 300), (512, 512, False, 2)])
+def test_rotated_rows_are_off_by_their_roundings_only(hip, hd, rot, interleaved, rows):  # noqa: F811
+    """Sine and cosine, with the magnitude, rounded to fp32 once, two products and a sum: 2 * 2^-24 (|x c| + |y s|) + 2^-24 of
+    the result, and the angle's own rounding (2^-53 of it; the fp64 restatement has the same).  A far position's angle of
+    2^24 rounded to fp32 as a fraction of a turn would be off by 1.9e-7 (|x| + |y|), wherever sine or cosine is small far more."""
+    rng = np.random.default_rng(hd + rows)
+    heads, kvh = 3, 1
+    cache = Cache(hip, rng, [4] * rows, 4, kvh, hd, False, True, fill=False)
+    x = rng.standard_normal((rows, heads + 2 * kvh, hd)).astype(np.float32)
+    pos = rng.integers(0, 1 << 24, rows).astype(np.int32)
+    pos[:2] = 0, -(1 << 24)
+    freq, mag = hipdec.rope_frequencies(rot, scaling=RopeScaling.PARTS, factor=8.0)
+    wide, d = (heads + 2 * kvh) * hd, hip.put(x)
+    d_out = hip.put(np.zeros((rows, heads, hd), np.float32))
+    hipdec.rope_append_paged(Rope.make(hip.put(freq), rot, interleaved=interleaved, magnitude=mag), cache.c, d, d + 4 * heads * hd,
+                             d + 4 * (heads + kvh) * hd, d_out, hip.put(pos), rows, heads, slots=hip.put(np.ones(rows, np.int32)), row_stride=wide)
+    hip.sync()
+    got = np.concatenate([fetch(hip, d_out, (rows, heads, hd), False), cache.down()[0][cache.table[:, 0], 1]], axis=1)
+    x = x[:, :heads + kvh]
+    want = turned(x, pos, freq, mag, rot, interleaved)
+    an = pos.astype(np.float64)[:, None, None] * freq
+    e, o = (slice(0, rot, 2), slice(1, rot, 2)) if interleaved else (slice(0, rot // 2), slice(rot // 2, rot))
+    ax, ay = np.abs(x[..., e].astype(np.float64)), np.abs(x[..., o].astype(np.float64))
+    c, s = np.abs(np.cos(an)) * mag, np.abs(np.sin(an)) * mag
+    tol = EPS * np.abs(want)
+    tol[..., rot:] = 0.0
+    for part, big in ((e, ax * c + ay * s), (o, ay * c + ax * s)):
+        tol[..., part] += 2.01 * EPS * big + (ax + ay) * mag * (np.abs(an) + 1) * 2.0 ** -52
+    assert np.all(np.abs(got - want) <= tol), (np.abs(got - want) / np.maximum(tol, 1e-30)).max()

@@ -78,3 +78,8 @@ def test_attention_counts_its_launches_as_they_are(kw, text):
     hd, dt = kw.pop("hd", 128), kw.pop("kv_dtype", KvDtype.BF16)
     c = PagedCache.make(FAKE, FAKE, dt, n_pages=4, page_size=16, kv_heads=8, hd=hd, page_table=FAKE, n_seqs=2, max_pages=2)
     refused(lambda: attention(cache=c, workspace=FAKE, workspace_bytes=HUGE, **kw), text)
+
+
+# ---------------------------------------------------------------- rotary positions
+def test_rotated_rows_are_off_by_their_roundings_only(emulated):
+    emulated("paged_edges", "rotation_roundings")
