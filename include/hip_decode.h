@@ -102,8 +102,9 @@ void hipdec_destroy(hipdec_model *m);
  * pays the weights once with this.) */
 int hipdec_create_shared(const hipdec_model *base, uint32_t kv_dtype, uint32_t flags, hipdec_model **out);
 
-/* Text of the last error on this model (or, when m is NULL, of the last failed call without a model on the
- * calling thread, hipdec_create among them). */
+/* Text of the last error on this model; when m is NULL, of the process's last failed call without a model (hipdec_create
+ * among them, whichever thread made it), or of the operator on device buffers (below) that failed on the calling thread, where
+ * none of those has failed on this thread since.  It stands until the calling thread asks again or fails again. */
 const char *hipdec_last_error(const hipdec_model *m);
 
 /* Model::len / Model::set_len, lib.rs:209-215 (set_len clamps to cfg.seq). */

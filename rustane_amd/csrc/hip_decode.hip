@@ -40,7 +40,24 @@ struct DevLayer {
     void *kc = nullptr, *vc = nullptr;
 };
 
-thread_local std::string g_create_error;   // (per thread: two threads may fail at once)
+// Texts of failed calls without a model (hipdec_last_error(NULL)).  Creating a model, and every other entry but the operators on the
+// caller's device buffers, leaves its text to the whole process: a program may create on one thread and report on another.
+// An operator's text is the calling thread's own (requests on several threads may fail at once) and stands there until
+// another call without a model fails on that thread.
+struct CreateError {
+    std::mutex mu;
+    std::string text;
+    CreateError &operator=(const std::string &what);
+};
+CreateError g_create_error;
+thread_local std::string g_op_error, g_shown_error;
+thread_local bool g_op_failed = false;
+CreateError &CreateError::operator=(const std::string &what) {
+    std::lock_guard<std::mutex> lock(mu);
+    g_op_failed = false;
+    text = what;
+    return *this;
+}
 
 // Workspace of the chunked prompt prefill (hipdec_prefill.h), allocated at the first prefill.
 struct PrefillWork {
@@ -1255,7 +1272,7 @@ int batch_fetch(hipdec_model *m, const void *dev, void *host, size_t floats) {
 
 // ---- requests of their own prompts stepped together over a paged cache (hipdec_requests.h)
 // an operator's refusal or failure as this model's
-#define OPCHK(expr) do { const int rc_ = (expr); if (rc_ != HIPDEC_OK) return fail(m, rc_, g_create_error.c_str()); } while (0)
+#define OPCHK(expr) do { const int rc_ = (expr); if (rc_ != HIPDEC_OK) { g_op_failed = false; return fail(m, rc_, g_op_error.c_str()); } } while (0)
 
 hipdec_paged_cache request_cache(const hipdec_model *m, uint32_t layer) {
     const RequestState &r = m->rq;
@@ -1532,11 +1549,20 @@ extern "C" {
 
 // errors of the entries without a model that live in other files (serving_ops.hip)
 __attribute__((visibility("hidden"))) int hipdec_op_error(int code, const char *entry, const char *what) {
-    try { g_create_error = std::string(entry) + ": " + what; } catch (...) { g_create_error.clear(); }
+    g_op_failed = true;
+    try { g_op_error = std::string(entry) + ": " + what; } catch (...) { g_op_error.clear(); }
     return code;
 }
 
-const char *hipdec_last_error(const hipdec_model *m) { return m ? m->err.c_str() : g_create_error.c_str(); }
+const char *hipdec_last_error(const hipdec_model *m) {
+    if (m) return m->err.c_str();
+    if (g_op_failed) return g_op_error.c_str();
+    try {                                                     // (a copy: another thread may fail while the caller reads)
+        std::lock_guard<std::mutex> lock(g_create_error.mu);
+        g_shown_error = g_create_error.text;
+    } catch (...) { g_shown_error.clear(); }
+    return g_shown_error.c_str();
+}
 
 void hipdec_destroy(hipdec_model *m) {
     if (!m) return;

@@ -1,11 +1,14 @@
 """Calls of the operators on the caller's device buffers that lie at the edge of what include/hip_decode.h allows, as far as no GPU
 is needed: the kernels' own source on the CPU under ASan (tests/kernel_emu/*_edges.cpp), one check per test."""
+import ctypes as C
 import os
 import re
 import subprocess
+import threading
 
 import pytest
 
+from rustane_amd import hipdec
 from rustane_amd.hipdec import KvDtype, PagedCache, RowDtype
 from test_kernel_emulation import EMU, ROOT, host_clang
 from test_serving_ops import FAKE, attention, refused, verify
@@ -83,3 +86,38 @@ def test_attention_counts_its_launches_as_they_are(kw, text):
 # ---------------------------------------------------------------- rotary positions
 def test_rotated_rows_are_off_by_their_roundings_only(emulated):
     emulated("paged_edges", "rotation_roundings")
+
+
+# ---------------------------------------------------------------- texts of failed calls
+def on_a_thread_of_its_own(call):
+    out = []
+    t = threading.Thread(target=lambda: out.append(call()))
+    t.start()
+    t.join()
+    return out[0]
+
+
+def test_any_thread_is_told_why_a_model_was_not_created():
+    lib = hipdec.load_library()
+    cfg, out = hipdec.Config.make(dim=64, hidden=64, heads=1, hd=64, seq=8, nlayers=2, vocab=8), C.c_void_p()
+    text = lambda: lib.hipdec_last_error(None)  # noqa: E731
+
+    def create(n_layers):
+        one = (C.c_float * 1)()
+        head = hipdec._Head(C.cast(one, C.POINTER(C.c_float)), C.cast(one, C.POINTER(C.c_float)))
+        layers = (hipdec._Layer * 1)()
+        return lib.hipdec_create(C.byref(cfg), layers, n_layers, C.byref(head), None, C.byref(out)), text()
+
+    # the creating thread, and one that has not failed in anything itself
+    rc, told = on_a_thread_of_its_own(lambda: create(7))
+    assert rc == hipdec.ERR_ARG and b"layer count" in told
+    assert b"layer count" in on_a_thread_of_its_own(text)
+    # an operator's failure is the failing thread's own: it hides neither the other's text nor, later, its own creation's
+    def operator_then_create():
+        refused(lambda: attention(scale=0.0), "scale")
+        mine, other = text(), on_a_thread_of_its_own(text)
+        on_a_thread_of_its_own(lambda: create(9))
+        return mine, other, text(), create(8)[1], on_a_thread_of_its_own(text)
+    mine, other, still, later, told = on_a_thread_of_its_own(operator_then_create)
+    assert b"scale" in mine and b"scale" in still and b"layer count" in other and b"layer count" in later and b"layer count" in told
+    assert not out.value
