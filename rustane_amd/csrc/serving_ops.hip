@@ -256,6 +256,7 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
     if (!aligned16(rows->d_q) || !aligned16(rows->d_out) || !aligned16(cache->k) || !aligned16(cache->v) ||
         (rows->q_stride | rows->out_stride) % row_unit || (cache->stride_page | cache->stride_slot | cache->stride_head) % kv_unit)
         return refuse(me, "queries, outputs and the cache must be 16-byte aligned, with strides of whole 16 bytes");
+    if (rows->n_rows > 1 && rows->d_q == rows->d_out && rows->q_stride != rows->out_stride) return refuse(me, "in place, both strides must be equal");
 
     const uint64_t slots = (uint64_t)cache->max_pages * cache->page_size;
     const bool qb = rows->dtype == HIPDEC_ROWS_BF16, cb = cache->kv_dtype == HIPDEC_KV_BF16;

@@ -121,3 +121,12 @@ def test_any_thread_is_told_why_a_model_was_not_created():
     mine, other, still, later, told = on_a_thread_of_its_own(operator_then_create)
     assert b"scale" in mine and b"scale" in still and b"layer count" in other and b"layer count" in later and b"layer count" in told
     assert not out.value
+
+
+# ---------------------------------------------------------------- one buffer for two things
+def test_attention_in_place_needs_one_stride():
+    wide = 8 * 128
+    refused(lambda: attention(q_stride=wide, out_stride=wide + 8), "in place")
+    refused(lambda: attention(q_stride=wide + 8, out_stride=wide), "in place")
+    refused(lambda: attention(q_stride=wide + 8, out_stride=wide + 8), "device")                  # (allowed; the address is no device memory)
+    refused(lambda: attention(n_rows=1, q_stride=wide + 8, out_stride=wide), "device")            # one row: no stride is used
