@@ -93,15 +93,16 @@ Split split_of(uint64_t n_rows, uint32_t kv_heads, uint32_t g, uint64_t max_len)
 }
 
 // Workspace for n_rows rows and max_len, and for anything smaller in either: with u key-head tiles per row, rows * splits
-// is at most rows * steps / 8 where the 1024 keys decide, and rows * (2 CUs / (rows u) + 1) where the CUs do.
-uint64_t attention_bytes(uint64_t n_rows, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint64_t max_len) {
+// is at most rows * steps / 8 where the 1024 keys decide, and rows * (2 CUs / (rows u) + 1) where the CUs do.  (No call whose
+// launches fit comes near 64 bits; the largest sizes that can be asked for pass them.)
+unsigned __int128 attention_bytes(uint64_t n_rows, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint64_t max_len) {
     if (max_len <= 256 || !n_rows) return 0;
     const uint64_t u = (uint64_t)kv_heads * ((heads / kv_heads + 15) / 16), steps = (max_len + 127) / 128;
     uint64_t most = n_rows * ((steps + 7) / 8);
     const uint64_t by_cus = (2 * kCus + u - 1) / u + n_rows;
     if (most < by_cus) most = by_cus;
     if (most > n_rows * steps) most = n_rows * steps;
-    return most * heads * (hd + 2) * sizeof(float);
+    return (unsigned __int128)(most * heads) * (hd + 2) * sizeof(float);
 }
 
 // Waves of a workgroup where one split writes the result (eight of the widest fp32 heads would not keep their registers).
@@ -233,7 +234,9 @@ int hipdec_attention_paged_workspace(uint64_t n_rows, uint32_t heads, uint32_t k
     if (!out_bytes) return refuse(me, "null argument");
     if (!heads || !kv_heads || heads % kv_heads || heads > 65536 || hd > kMaxHeadDim || n_rows > kMaxRows || max_len > kMaxLen)
         return refuse(me, "heads, hd, n_rows or max_len out of range");
-    *out_bytes = attention_bytes(n_rows, heads, kv_heads, hd, max_len);
+    const unsigned __int128 bytes = attention_bytes(n_rows, heads, kv_heads, hd, max_len);
+    if (bytes >> 64) return refuse(me, "n_rows * heads * max_len out of range");
+    *out_bytes = (uint64_t)bytes;
     return HIPDEC_OK;
 }
 

@@ -130,3 +130,15 @@ def test_attention_in_place_needs_one_stride():
     refused(lambda: attention(q_stride=wide + 8, out_stride=wide), "in place")
     refused(lambda: attention(q_stride=wide + 8, out_stride=wide + 8), "device")                  # (allowed; the address is no device memory)
     refused(lambda: attention(n_rows=1, q_stride=wide + 8, out_stride=wide), "device")            # one row: no stride is used
+
+
+def test_a_workspace_past_64_bits_is_refused_not_wrapped():
+    sizes = []
+    for n_rows, heads, kv_heads, hd, max_len in ((1 << 24, 65536, 1, 512, 1 << 30), (1 << 24, 65536, 65536, 512, 1 << 30), (1 << 24, 65536, 1, 510, 1 << 29)):
+        refused(lambda: hipdec.attention_paged_workspace(n_rows, heads, kv_heads, hd, max_len), "out of range")
+    for shift in range(0, 25):                               # up to there it grows with the rows
+        try:
+            sizes.append(hipdec.attention_paged_workspace(1 << shift, 65536, 8, 256, 1 << 26))
+        except hipdec.HipDecodeError:
+            sizes.append(1 << 64)
+    assert sizes == sorted(sizes) and sizes[12] < 1 << 64
