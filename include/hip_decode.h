@@ -215,7 +215,8 @@ int hipdec_requests_len(const hipdec_model *m, uint32_t seq, size_t *out_len, si
  * The decision is hipdec_verify_drafts' with host arrays: draft_probs[n_seqs][max_drafts][vocab] (NULL: the drafts
  * are certain), uniforms[n_seqs][max_drafts + 1] in [0, 1) (may be NULL with temperature 0).
  * out_tokens[n_seqs][max_drafts + 1]: the kept drafts, the next token (to be fed in the next step), then 0xffffffff;
- * out_accepted[n_seqs]: how many drafts were kept.  The sequence grows by its token and the kept drafts.
+ * out_accepted[n_seqs]: how many drafts were kept.  The sequence grows by its token and the kept drafts; pages
+ * that only drafts that were not kept had needed go back to the pool.
  * out_logits (nullable): [n_seqs][max_drafts + 1][vocab] raw logits, rows behind a sequence's drafts meaningless.
  * HIPDEC_ERR_FULL, with nothing changed, where a sequence would pass cfg.seq or the pool has too few free pages. */
 int hipdec_requests_step(hipdec_model *m, size_t n_seqs, const uint32_t *seqs, const uint32_t *tokens, uint32_t max_drafts,

@@ -1350,6 +1350,23 @@ size_t request_pages_missing(const hipdec_model *m, uint32_t q, size_t len) {
     for (size_t p = 0; p << r.page_shift < len; ++p) n += row[p] < 0;
     return n;
 }
+// Gives back what sequences hold beyond their lengths, whichever way the call that took pages for them ends: the pages that only
+// rejected drafts were written to, and those of a step or an admission that failed.  (The device's table keeps their
+// numbers behind the length, where no row looks, until the sequence's next step.  Last page first: the next one given is it.)
+struct RequestTrim {
+    hipdec_model *m;
+    const uint32_t *seqs;
+    size_t n;
+    ~RequestTrim() {
+        RequestState &r = m->rq;
+        for (size_t i = 0; i < n; ++i) {
+            int *row = &r.table[(size_t)seqs[i] * r.max_pages];
+            const long long len = std::max(r.lens[seqs[i]], 0LL);
+            for (int p = r.max_pages - 1; p >= 0 && (long long)p << r.page_shift >= len; --p)
+                if (row[p] >= 0) { r.free_pages.push_back(row[p]); row[p] = -1; }
+        }
+    }
+};
 int request_table_up(hipdec_model *m, uint32_t q) {
     RequestState &r = m->rq;
     const size_t at = (size_t)q * r.max_pages;
@@ -2401,6 +2418,7 @@ int hipdec_requests_admit(hipdec_model *m, uint32_t seq) {
     if (request_pages_missing(m, seq, m->len) > r.free_pages.size()) return fail(m, HIPDEC_ERR_FULL, "not enough free pages");
     HCHK(hipSetDevice(m->opt.device));
     HCHK(hipStreamSynchronize(m->stream));
+    const RequestTrim trim{m, &seq, 1};
     request_pages(m, seq, m->len);
     const int rc = request_table_up(m, seq);
     if (rc) return rc;
@@ -2472,6 +2490,7 @@ int hipdec_requests_step(hipdec_model *m, size_t n_seqs, const uint32_t *seqs, c
     if (draft_probs && K && temperature > 0.0f && !r.d_probs && (rc = dalloc(m, &r.d_probs, (size_t)kRequestRows * c.vocab * 4))) return rc;
     PrefillWork &w = m->pf;
     HCHK(hipStreamSynchronize(m->stream));                      // pinned staging is free again
+    const RequestTrim trim{m, seqs, n_seqs};
     int *pos = r.h_rows, *slot = pos + kRequestRows, *sq = slot + kRequestRows, *ln = sq + kRequestRows, *dr = ln + kRequestRows, *nn = dr + kRequestRows;
     for (size_t i = 0; i < n_seqs; ++i) {
         const size_t nd = n_drafts ? n_drafts[i] : K, len = (size_t)r.lens[seqs[i]];

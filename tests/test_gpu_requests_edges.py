@@ -1,0 +1,48 @@
+"""Requests stepped together (hipdec_requests_*) at the edge of what include/hip_decode.h allows."""
+import numpy as np
+import pytest
+
+from rustane_amd import hipdec
+from rustane_amd.hipdec import HipDecodeError, KvDtype, NO_TOKEN
+from test_gpu_requests import admit, alone, close, model
+
+pytestmark = pytest.mark.gpu
+
+
+def test_rejected_drafts_give_their_pages_back():
+    m = model(kd=KvDtype.BF16)
+    rng = np.random.default_rng(8)
+    prompt = rng.integers(0, 700, 4)
+    m.requests_open(4, 9, 3)
+    for s in (0, 1):
+        admit(m, s, prompt)                                  # a page each, full
+    assert m.requests_len(0) == (4, 7)
+    first = int(m.requests_step([1], [3])[0][0, 0])          # what follows, without drafts
+    assert m.requests_len(1) == (5, 6)
+    # twelve drafts of which the first is wrong: positions 4 .. 16 are written, one stays
+    drafts = [[(first + 1) % 700] + [7] * 11]
+    out, acc = m.requests_step([0], [3], drafts=drafts)
+    assert acc[0] == 0 and out[0, 0] == first and np.all(out[0, 1:] == NO_TOKEN)
+    assert m.requests_len(0) == (5, 5)                       # two pages each; five are left
+    # the rest of the pool serves a third request of the length that just fits, and the first one goes on as if alone
+    admit(m, 2, rng.integers(0, 700, 19))
+    assert m.requests_len(2) == (19, 0)
+    got = [m.requests_step([0], [t], logits=True)[2][0, 0] for t in (first, 9, 11)]
+    close(np.stack(got), alone(m, prompt, [3, first, 9, 11])[1:], 2e-2)
+    assert m.requests_len(0) == (8, 0)
+    with pytest.raises(HipDecodeError) as e:
+        m.requests_step([0], [1])
+    assert e.value.status == hipdec.ERR_FULL and m.requests_len(0) == (8, 0)
+    # partly kept drafts: what is kept stays, what lies behind it goes back
+    for s in (0, 1, 2):
+        m.requests_release(s)
+    admit(m, 1, prompt)
+    stream, tok = [], 3
+    for _ in range(4):
+        tok = int(m.requests_step([1], [tok])[0][0, 0])
+        stream.append(tok)
+    m.requests_release(1)
+    admit(m, 0, prompt)
+    out, acc = m.requests_step([0], [3], drafts=[stream[:2] + [(stream[2] + 1) % 700] + [5] * 10])
+    assert acc[0] == 2 and out[0, :3].tolist() == stream[:3]
+    assert m.requests_len(0) == (7, 7)
