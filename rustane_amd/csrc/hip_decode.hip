@@ -788,7 +788,8 @@ int pf_ensure(hipdec_model *m, int T, bool with_head = false) {
     PrefillWork &w = m->pf;
     int rc;
     if (w.rows < T) {
-        const size_t R = (size_t)std::min<size_t>(kPrefillMaxRows, c.seq);
+        // (a step of samples or requests has up to kRequestRows rows, also where the window has fewer positions)
+        const size_t R = std::max<size_t>(std::min<size_t>(kPrefillMaxRows, c.seq), kRequestRows);
         if ((rc = dalloc(m, &w.ids, R * 4))) return rc;
         if ((rc = dalloc(m, &w.x, R * D * 4))) return rc;
         if ((rc = dalloc(m, &w.x2, R * D * 4))) return rc;
@@ -962,6 +963,7 @@ int prefill_batched(hipdec_model *m, const uint32_t *ids, size_t n, const float 
 
 // ---- multi-sample decode (hipdec_batch.h)
 constexpr int kBatchMaxRows = 32;
+static_assert(kBatchMaxRows <= kRequestRows, "pf_ensure makes room for both");
 
 int batch_alloc(hipdec_model *m, int rows) {
     const hipdec_config &c = m->cfg;
@@ -2466,7 +2468,7 @@ int hipdec_requests_step(hipdec_model *m, size_t n_seqs, const uint32_t *seqs, c
     if (!(temperature >= 0.0f) || !std::isfinite(temperature) || !(softcap <= 3.4e38f)) return fail(m, HIPDEC_ERR_ARG, "temperature must not be negative, softcap must be finite");
     if (temperature > 0.0f && !uniforms) return fail(m, HIPDEC_ERR_ARG, "random numbers are missing");
     const size_t K = max_drafts, S = K + 1;
-    if (n_seqs == 0 || n_seqs > (size_t)kRequestRows || S > (size_t)kRequestRows || n_seqs * S > (size_t)kRequestRows || n_seqs * S > c.seq)
+    if (n_seqs == 0 || n_seqs > (size_t)kRequestRows || S > (size_t)kRequestRows || n_seqs * S > (size_t)kRequestRows)
         return fail(m, HIPDEC_ERR_ARG, "n_seqs * (max_drafts + 1) must be in 1..32");
     size_t missing = 0, max_len = 0;
     for (size_t i = 0; i < n_seqs; ++i) {

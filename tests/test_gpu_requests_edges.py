@@ -46,3 +46,30 @@ def test_rejected_drafts_give_their_pages_back():
     out, acc = m.requests_step([0], [3], drafts=[stream[:2] + [(stream[2] + 1) % 700] + [5] * 10])
     assert acc[0] == 2 and out[0, :3].tolist() == stream[:3]
     assert m.requests_len(0) == (7, 7)
+
+
+@pytest.mark.parametrize("seq,n", [(16, 20), (8, 32)])
+def test_more_rows_than_the_window_has_positions(seq, n):
+    m = model(seq=seq)
+    rng = np.random.default_rng(9)
+    prompts = [rng.integers(0, 700, i % (seq - 2)) for i in range(n)]
+    m.requests_open(4, n * seq // 4, n)
+    for s, p in enumerate(prompts):
+        admit(m, s, p)
+    fed = rng.integers(0, 700, (n, 2))
+    seen = [m.requests_step(np.arange(n), fed[:, t], logits=True)[2][:, 0] for t in range(2)]
+    for s in range(n):
+        close(np.stack([x[s] for x in seen]), alone(m, prompts[s], fed[s]), 2e-3)
+
+
+def test_more_samples_than_the_window_has_positions():
+    m = model(seq=16)
+    rng = np.random.default_rng(10)
+    prompt, fed = rng.integers(0, 700, 5), rng.integers(0, 700, 24)
+    want = np.concatenate([alone(m, prompt, [t]) for t in fed])
+    m.set_len(0)
+    m.prefill(np.asarray(prompt, np.uint32))
+    m.batch_begin(24)
+    got = m.decode_logits_from_ids_batch(np.asarray(fed, np.uint32))
+    m.batch_end()
+    close(np.asarray(got).reshape(24, -1), want, 2e-3)
