@@ -2450,7 +2450,10 @@ int hipdec_requests_release(hipdec_model *m, uint32_t seq) {
 }
 
 int hipdec_requests_len(const hipdec_model *m, uint32_t seq, size_t *out_len, size_t *out_free_pages) {
-    if (!m || !m->rq.open || seq >= m->rq.max_seqs || m->rq.lens[seq] < 0) return HIPDEC_ERR_ARG;
+    if (!m) return HIPDEC_ERR_ARG;
+    hipdec_model *told = const_cast<hipdec_model *>(m);       // (its error text only)
+    if (!m->rq.open) return fail(told, HIPDEC_ERR_ARG, "no pages are open (hipdec_requests_open)");
+    if (seq >= m->rq.max_seqs || m->rq.lens[seq] < 0) return fail(told, HIPDEC_ERR_ARG, "no such sequence");
     if (out_len) *out_len = (size_t)m->rq.lens[seq];
     if (out_free_pages) *out_free_pages = m->rq.free_pages.size();
     return HIPDEC_OK;

@@ -73,3 +73,15 @@ def test_more_samples_than_the_window_has_positions():
     got = m.decode_logits_from_ids_batch(np.asarray(fed, np.uint32))
     m.batch_end()
     close(np.asarray(got).reshape(24, -1), want, 2e-3)
+
+
+def test_lengths_of_no_sequence_say_so():
+    m = model()
+    with pytest.raises(HipDecodeError) as e:
+        m.requests_len(0)
+    assert "no pages are open" in str(e.value)
+    m.requests_open(8, 4, 2)
+    for s in (0, 5):
+        with pytest.raises(HipDecodeError) as e:
+            m.requests_len(s)
+        assert "no such sequence" in str(e.value)
