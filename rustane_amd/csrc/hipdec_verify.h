@@ -127,6 +127,9 @@ __device__ __forceinline__ double vf_exp2(double y) {
 // softcap(x) / cap = tanh(x / cap) = E / (E + 2) with E = e^(2 x / cap) - 1 = 2^n (2^f - 1) + (2^n - 1): nothing cancels, so
 // it is right to 1e-14 of itself, at a cap far above the logits too.  Past 2^+-100 it is +-1.  (The plain form without cap.)
 template <bool CAP> __device__ __forceinline__ double vf_capped(const VerifyArgs &a, float x) {
+    // (the last product stays a number of its own: fused into the difference of two caps, as this compiler does where it may, a
+    // logit's difference to itself would be that product's rounding, not 0, and a tiny temperature makes that the whole weight)
+#pragma clang fp contract(off)
     if (!CAP) return (double)x;
     const float far = 34.657359f * (float)a.cap;             // 100 of 2 log2(e) / cap
     uint32_t n;

@@ -5,7 +5,7 @@ import pytest
 
 from rustane_amd import hipdec
 from rustane_amd.hipdec import Rope, RopeScaling
-from test_gpu_serving_ops import EPS, Cache, fetch, hip, turned  # noqa: F401
+from test_gpu_serving_ops import EPS, Cache, Rows, attend, attended, draft_case, fetch, hip, turned, verified, verify  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,19 @@ def test_rotated_rows_are_off_by_their_roundings_only(hip, hd, rot, interleaved,
     for part, big in ((e, ax * c + ay * s), (o, ay * c + ax * s)):
         tol[..., part] += 2.01 * EPS * big + (ax + ay) * mag * (np.abs(an) + 1) * 2.0 ** -52
     assert np.all(np.abs(got - want) <= tol), (np.abs(got - want) / np.maximum(tol, 1e-30)).max()
+
+
+@pytest.mark.parametrize("T", [1e-12, 1e-18, 1e-20, 1e-30, 1.2e-38])
+def test_tiny_temperatures_with_a_saturated_soft_cap(hip, T):  # noqa: F811
+    """Logits of twenty caps and more are within the last bits of each other: only one of them may be kept or drawn."""
+    rng = np.random.default_rng(15)
+    S, K, V = 16, 3, 3000
+    x = rng.standard_normal((S, K + 1, V)).astype(np.float32)
+    x[..., 1::2] = 40.0 + 30.0 * rng.random((S, K + 1, V // 2), dtype=np.float32)
+    drafts, n = rng.integers(0, V, (S, K)).astype(np.int32), np.full(S, K, np.int32)
+    probs = np.full((S, K, V), 1.0 / V, np.float32)
+    for p in (probs, None):
+        tokens, accepted = verify(hip, Rows(x, False), drafts, n, rng.random((S, K + 1), dtype=np.float32), T, 2.0, p)
+        for s in range(S):
+            kept = tokens[s, :accepted[s] + 1]
+            assert np.all(kept < V) and np.all(kept % 2 == 1) and np.all(tokens[s, accepted[s] + 1:] == hipdec.NO_TOKEN), (tokens[s], accepted[s])

@@ -24,11 +24,13 @@ def emulated(tmp_path_factory):
         text = open(os.path.join(ROOT, "rustane_amd", "csrc", "hipdec_%s.h" % name)).read()
         (build / ("kernel_%s.inc" % name)).write_text(re.sub(r"^#(pragma once|include .*)$", "", text, flags=re.M))
     built = {}
+    # products and sums fused where the GPU's compiler fuses them, if this machine can
+    fused = ["-mfma", "-ffp-contract=fast-honor-pragmas"] if re.search(r"^flags.* fma ", open("/proc/cpuinfo").read(), re.M) else []
 
     def check(program, name):
         if program not in built:
             cmd = [cxx, "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=undefined",
-                   "-fno-omit-frame-pointer", "-pthread", "-Wno-psabi", "-I", str(build), "-I", EMU,
+                   "-fno-omit-frame-pointer", "-pthread", "-Wno-psabi", *fused, "-I", str(build), "-I", EMU,
                    os.path.join(EMU, program + ".cpp"), "-o", str(build / program)]
             r = subprocess.run(cmd, capture_output=True, text=True)
             assert r.returncode == 0, r.stderr[-4000:]
