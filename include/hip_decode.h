@@ -420,7 +420,7 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
  * number is used (d_uniforms may be NULL).
  *   d_tokens[s][max_drafts + 1]: the kept drafts, the next token, then 0xffffffff; d_accepted[s]: how many drafts
  * were kept.  A draft outside the vocabulary is not kept; logits that are NaN or -inf are impossible tokens, and a row
- * of nothing else gives the next token 0xffffffff.  A negative random number or draft probability counts as 0, a draft is
+ * of nothing else gives the next token 0xffffffff; logits of +inf share the whole (with the largest finite fp32 number).  A negative random number or draft probability counts as 0, a draft is
  * not kept where either is a NaN, and a NaN probability leaves its token nothing of max(p - q, 0).
  *   softcap <= 0: none.  vocab <= 262144, max_drafts 0 .. 255.
  *   d_workspace: at least hipdec_verify_drafts_workspace bytes (which also serve fewer sequences, fewer drafts and a

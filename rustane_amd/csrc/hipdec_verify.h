@@ -44,10 +44,11 @@ struct VerifyArgs {
 __device__ __forceinline__ int vf_drafts(const VerifyArgs &a, int s) {
     return a.n_drafts ? min(max(a.n_drafts[s], 0), a.max_drafts) : a.max_drafts;
 }
-// stored logit as a number: a NaN is no possible token; infinite ones share the whole
-template <bool B16> __device__ __forceinline__ float vf_number(uint32_t raw) {
+// stored logit as a number: a NaN is no possible token; infinite ones share the whole, and at temperature 0 are the largest
+__device__ __forceinline__ float vf_most(const VerifyArgs &a) { return a.k > 0.0 ? 3.4028235e38f : INFINITY; }
+template <bool B16> __device__ __forceinline__ float vf_number(uint32_t raw, float most) {
     const float x = B16 ? bf16_to_f32(raw) : __uint_as_float(raw);
-    return fminf(x == x ? x : -INFINITY, 3.4028235e38f);
+    return fminf(x == x ? x : -INFINITY, most);
 }
 template <bool B16> __device__ __forceinline__ uint32_t vf_raw(const void *row, int i) {
     return B16 ? ((const uint16_t *)row)[i] : ((const uint32_t *)row)[i];
@@ -56,7 +57,7 @@ template <bool B16> __device__ __forceinline__ const void *vf_row_of(const Verif
     return B16 ? (const void *)((const uint16_t *)a.logits + row * a.row_stride) : (const void *)((const float *)a.logits + row * a.row_stride);
 }
 template <bool B16> __device__ __forceinline__ float vf_logit(const VerifyArgs &a, long long row, int i) {
-    return vf_number<B16>(vf_raw<B16>(vf_row_of<B16>(a, row), i));
+    return vf_number<B16>(vf_raw<B16>(vf_row_of<B16>(a, row), i), vf_most(a));
 }
 // PER logits of a lane: those of its wave's chunk 64 apart, or neighbours; -inf behind the vocabulary.  (All of them are
 // asked for before the first is looked at; the chunk is the same for the whole wave, and so is the question whether it
@@ -65,17 +66,18 @@ template <bool B16> __device__ __forceinline__ float vf_logit(const VerifyArgs &
 template <bool B16, int PER, bool NEAR> __device__ __forceinline__ void vf_logits(const VerifyArgs &a, long long row, int chunk, float *x) {
     const int first = chunk * PER * WAVE, lane = threadIdx.x & 63, step = NEAR ? 1 : WAVE, mine = first + (NEAR ? lane * PER : lane);
     const void *p = vf_row_of<B16>(a, row);
+    const float most = vf_most(a);
     uint32_t raw[PER];
     if (first + PER * WAVE <= a.vocab) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) raw[i] = vf_raw<B16>(p, mine + i * step);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) x[i] = vf_number<B16>(raw[i]);
+        for (int i = 0; i < PER; ++i) x[i] = vf_number<B16>(raw[i], most);
     } else {
 #pragma unroll
         for (int i = 0; i < PER; ++i) raw[i] = vf_raw<B16>(p, min(mine + i * step, a.vocab - 1));
 #pragma unroll
-        for (int i = 0; i < PER; ++i) x[i] = mine + i * step < a.vocab ? vf_number<B16>(raw[i]) : -INFINITY;
+        for (int i = 0; i < PER; ++i) x[i] = mine + i * step < a.vocab ? vf_number<B16>(raw[i], most) : -INFINITY;
     }
 }
 // a probability of the draft's, or a random number, as it counts: a negative one is 0 (a token that the target cannot give, or that

@@ -183,6 +183,25 @@ static int tiny_temperatures() {
     return wrong;
 }
 
+// Temperature 0: an infinite logit is above the largest finite one, and the first of equals is taken; drafts among them.
+static int greedy_infinities() {
+    int wrong = 0;
+    for (float cap : {0.0f, 4.0f}) {
+        Drafts c(5, 2, 1500, 0.0f, cap, true);
+        for (int s = 0; s < c.S; ++s)
+            for (int i = 0; i <= c.K; ++i) {
+                float *x = c.row(s, i);
+                x[3] = 3.4028235e38f;
+                if (s) x[500] = x[1400] = INFINITY;
+                if (s == 2) x[40] = INFINITY;
+                if (s == 3) for (int j = 0; j < c.V; ++j) x[j] = j % 2 ? -INFINITY : NAN;
+                if (i < c.K) c.d[s * c.K + i] = s == 0 ? 3 : s == 1 ? (i ? 1400 : 500) : s == 2 ? 40 : s == 3 ? 1 : 3;
+            }
+        wrong += compared(cap > 0 ? "soft cap" : "no cap", cap > 0 ? run<true, 4>(c) : run<false, 4>(c), wanted(c));
+    }
+    return wrong;
+}
+
 // The soft cap and the exponential against long double.  Allowed: the polynomial's 1.5e-15, the reciprocal's 2^-48 = 3.6e-15 behind
 // one Newton step and some ten roundings of 1.1e-16: 1e-14 of the value; the exponential, without a reciprocal, 4e-15.
 static int elementary_accuracy() {
@@ -209,7 +228,7 @@ static int elementary_accuracy() {
 
 int main(int argc, char **argv) {
     const struct { const char *name; int (*check)(); } checks[] = {{"negative_numbers", negative_numbers}, {"tiny_temperatures", tiny_temperatures},
-                                                               {"elementary_accuracy", elementary_accuracy}};
+                                                               {"elementary_accuracy", elementary_accuracy}, {"greedy_infinities", greedy_infinities}};
     for (const auto &c : checks)
         if (argc > 1 && !std::strcmp(argv[1], c.name)) {
             const int wrong = c.check();

@@ -56,3 +56,15 @@ def test_tiny_temperatures_with_a_saturated_soft_cap(hip, T):  # noqa: F811
         for s in range(S):
             kept = tokens[s, :accepted[s] + 1]
             assert np.all(kept < V) and np.all(kept % 2 == 1) and np.all(tokens[s, accepted[s] + 1:] == hipdec.NO_TOKEN), (tokens[s], accepted[s])
+
+
+@pytest.mark.parametrize("cap", [0.0, 4.0])
+def test_an_infinite_logit_is_the_largest_at_temperature_zero(hip, cap):  # noqa: F811
+    rng = np.random.default_rng(16)
+    x = rng.standard_normal((4, 2, 1500)).astype(np.float32)
+    x[..., 3] = np.finfo(np.float32).max
+    x[1:, :, 500] = x[1:, :, 1400] = np.inf
+    x[2, :, 40] = np.inf
+    drafts = np.array([[3], [500], [40], [3]], np.int32)
+    tokens, accepted = verify(hip, Rows(x, False), drafts, np.ones(4, np.int32), np.zeros((4, 2), np.float32), 0.0, cap)
+    assert accepted.tolist() == [1, 1, 1, 0] and tokens.tolist() == [[3, 3], [500, 500], [40, 40], [500, hipdec.NO_TOKEN]]

@@ -53,6 +53,10 @@ def test_soft_cap_and_exponential_are_right_to_64_bits(emulated):
     emulated("verify_edges", "elementary_accuracy")
 
 
+def test_an_infinite_logit_is_the_largest_at_temperature_zero(emulated):
+    emulated("verify_edges", "greedy_infinities")
+
+
 # ---------------------------------------------------------------- sizes at the launches' limits (no GPU: the host decides)
 HUGE = 1 << 62                # workspace bytes
 
