@@ -149,7 +149,7 @@ template <bool CAP, bool EXACT_ZERO> __device__ __forceinline__ double vf_weight
     // (the cap's last bits can put a logit that it saturates above the maximum's, which a small temperature multiplies without limit)
     if (CAP) y = fmin(y, 0.0);
     const double w = vf_exp2(y);
-    if (CAP) return x == -INFINITY ? 0.0 : w;
+    if (CAP && x == -INFINITY) return 0.0;
     return EXACT_ZERO ? y > -1021.0 ? w : 0.0 : w;
 }
 // max(p - q, 0), a NaN in q leaves 0.  (One fused operation wherever it is taken: a chunk whose sum is above 0 holds a

@@ -202,6 +202,26 @@ static int greedy_infinities() {
     return wrong;
 }
 
+// A soft cap and a small temperature: what lies too far below the maximum for 64 bits has no probability at all, as without a cap.
+// A random number of 0 finds the first token that has one, and a draft that covers those leaves no rest.
+static int far_below_the_maximum() {
+    int wrong = 0;
+    for (float cap : {0.0f, 30.0f})
+        for (bool with_probs : {true, false}) {
+            Drafts c(4, 2, 600, 1e-3f, cap, with_probs);
+            for (int s = 0; s < c.S; ++s)
+                for (int i = 0; i <= c.K; ++i) {
+                    for (int j = 0; j < c.V; ++j) c.row(s, i)[j] = j < 100 || j % 3 == 0 ? -30.0f : 25.0f + normal(1e-3f);
+                    for (int j = 0; i < c.K && j < c.V; ++j) c.prob(s, i)[j] = s == 3 || j == 101 ? 0.0f : 1.0f;
+                    if (i < c.K) { c.d[s * c.K + i] = s == 2 ? 7 : 400; c.u[s * 3 + i] = s == 2 ? 0.0f : 0.9f; }
+                    if (s == 1) for (int j = 0; i < c.K && j < c.V; ++j) c.prob(s, i)[j] = j < 100 ? 0.0f : 1.0f;
+                }
+            c.u[2] = c.u[11] = 0.0f;
+            wrong += compared(cap > 0 ? "soft cap" : "no cap", cap > 0 ? run<true, 4>(c) : run<false, 4>(c), wanted(c));
+        }
+    return wrong;
+}
+
 // The soft cap and the exponential against long double.  Allowed: the polynomial's 1.5e-15, the reciprocal's 2^-48 = 3.6e-15 behind
 // one Newton step and some ten roundings of 1.1e-16: 1e-14 of the value; the exponential, without a reciprocal, 4e-15.
 static int elementary_accuracy() {

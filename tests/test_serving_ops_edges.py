@@ -57,6 +57,10 @@ def test_an_infinite_logit_is_the_largest_at_temperature_zero(emulated):
     emulated("verify_edges", "greedy_infinities")
 
 
+def test_what_lies_too_far_below_the_maximum_has_no_probability(emulated):
+    emulated("verify_edges", "far_below_the_maximum")
+
+
 # ---------------------------------------------------------------- sizes at the launches' limits (no GPU: the host decides)
 HUGE = 1 << 62                # workspace bytes
 
