@@ -202,6 +202,19 @@ static int greedy_infinities() {
     return wrong;
 }
 
+// Eight logits a lane (chunks of 512), the form of 4 to 12 million logits and of vocabularies of 65537 .. 131072: several chunks,
+// the last one ending inside, and one chunk.
+static int eight_logits_a_lane() {
+    int wrong = 0;
+    for (int V : {4700, 1537, 300})
+        for (bool with_probs : {true, false}) {
+            Drafts c(7, 3, V, 0.8f, 0.0f, with_probs), d(7, 2, V, 1.1f, 12.0f, with_probs), e(4, 2, V, 0.0f, 0.0f, with_probs);
+            c.n = {3, 0, 1, 2, 3, 9, -1};
+            wrong += compared("no cap", run<false, 8>(c), wanted(c)) + compared("soft cap", run<true, 8>(d), wanted(d)) + compared("temperature 0", run<false, 8>(e), wanted(e));
+        }
+    return wrong;
+}
+
 // A soft cap and a small temperature: what lies too far below the maximum for 64 bits has no probability at all, as without a cap.
 // A random number of 0 finds the first token that has one, and a draft that covers those leaves no rest.
 static int far_below_the_maximum() {
@@ -248,7 +261,8 @@ static int elementary_accuracy() {
 
 int main(int argc, char **argv) {
     const struct { const char *name; int (*check)(); } checks[] = {{"negative_numbers", negative_numbers}, {"tiny_temperatures", tiny_temperatures},
-                                                               {"elementary_accuracy", elementary_accuracy}, {"greedy_infinities", greedy_infinities}};
+                                                               {"elementary_accuracy", elementary_accuracy}, {"greedy_infinities", greedy_infinities},
+                                                               {"eight_logits_a_lane", eight_logits_a_lane}, {"far_below_the_maximum", far_below_the_maximum}};
     for (const auto &c : checks)
         if (argc > 1 && !std::strcmp(argv[1], c.name)) {
             const int wrong = c.check();

@@ -61,6 +61,10 @@ def test_what_lies_too_far_below_the_maximum_has_no_probability(emulated):
     emulated("verify_edges", "far_below_the_maximum")
 
 
+def test_verification_with_eight_logits_a_lane(emulated):
+    emulated("verify_edges", "eight_logits_a_lane")
+
+
 # ---------------------------------------------------------------- sizes at the launches' limits (no GPU: the host decides)
 HUGE = 1 << 62                # workspace bytes
 
