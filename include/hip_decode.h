@@ -389,7 +389,9 @@ int hipdec_rope_append_paged(const hipdec_rope *rope, const hipdec_paged_cache *
  * exist are left out.  scale > 0.  hd: 64, 128, 192 or 256 (else HIPDEC_ERR_UNSUPPORTED); d_q, d_out and the
  * cache 16-byte aligned with strides that are multiples of 16 bytes.  d_workspace: at least
  * hipdec_attention_paged_workspace bytes (which also serve fewer rows and any smaller max_len), 16-byte aligned
- * (may be NULL if that is 0).  d_out may be d_q with the same stride, and must not overlap it otherwise. */
+ * (may be NULL if that is 0).  d_out may be d_q with the same stride, and must not overlap it otherwise.
+ * n_rows and max_len decide how a cache is split, so a row's last bits may differ with them; with both the same its result
+ * is its own, whatever the other rows are. */
 typedef struct {
     const void *d_q;
     void *d_out;
@@ -420,8 +422,9 @@ int hipdec_attention_paged(const hipdec_paged_cache *cache, const hipdec_attenti
  * number is used (d_uniforms may be NULL).
  *   d_tokens[s][max_drafts + 1]: the kept drafts, the next token, then 0xffffffff; d_accepted[s]: how many drafts
  * were kept.  A draft outside the vocabulary is not kept; logits that are NaN or -inf are impossible tokens, and a row
- * of nothing else gives the next token 0xffffffff; logits of +inf share the whole (with the largest finite fp32 number).  A negative random number or draft probability counts as 0, a draft is
- * not kept where either is a NaN, and a NaN probability leaves its token nothing of max(p - q, 0).
+ * of nothing else gives the next token 0xffffffff; logits of +inf share the whole (with those of the largest finite fp32
+ * number).  A negative random number or draft probability counts as 0, a draft is not kept where either is a NaN, and a
+ * NaN probability leaves its token nothing of max(p - q, 0).
  *   softcap <= 0: none.  vocab <= 262144, max_drafts 0 .. 255.
  *   d_workspace: at least hipdec_verify_drafts_workspace bytes (which also serve fewer sequences, fewer drafts and a
  * smaller vocabulary), 16-byte aligned. */

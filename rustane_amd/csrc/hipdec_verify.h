@@ -9,10 +9,10 @@
 //
 // Exponentials and sums are 64 bits wide: a token is decided where a running sum over up to a few hundred thousand
 // terms passes a border, and with fp32 sums (1e-7 of the whole) about one draw in a hundred would fall on another
-// token than the definition's; with 64 bits it is one in 1e8.
-// Measured (MI355X): one sequence of four looked-up drafts over 32768 tokens 10.2 us of kernels; 32 of up to 7 drafts with
-// probabilities 17.0 us; 64 of up to 5 over 131071 bf16 logits with a soft cap 80 us, where a vector instruction issues in
-// 98 % of the statistics' cycles (55 per logit, 34 of them 64 bits wide).
+// token than the definition's; with 64 bits it is one in 1e8 (with a soft cap, whose 1e-14 a temperature divides, at most one in 1e7).
+// Measured (MI355X): one sequence of four looked-up drafts over 32768 tokens 10.4 us of kernels; 32 of up to 7 drafts with
+// probabilities 17.7 us; 64 of up to 5 over 131071 bf16 logits with a soft cap 82 us, where a vector instruction issues in
+// 98 % of the statistics' cycles (60 per logit, 38 of them 64 bits wide).  At temperature 0, two launches, 5.8 / 9.9 / 20.7 us.
 #pragma once
 #include "hipdec_wave64.h"
 

@@ -126,8 +126,9 @@ template <bool RB, bool CB> hipError_t go_rope(const RopeArgs &a, bool wide, uin
 }
 
 // Logits of a row per wave: 256, 512 or 1024.  Few logits are latency, many are instructions, of which a chunk's maximum
-// and sum, and reading its statistics back, are a smaller part the more logits it has: 160 rows of 32768 17.2 / 16.6 /
-// 18.2 us, 512 rows 35.2 / 29.0 / 29.5, 256 rows of 131071 - / 53.5 / 49.9.  At most 256 chunks.
+// and sum, and reading its statistics back, are a smaller part the more logits it has: 20 rows of 32768 13.3 / 13.2 / 14.0 us, 160 rows
+// 17.5 / 16.7 / 18.1, 320 rows 27.6 / 23.1 / 22.9, 512 rows 36.1 / 30.1 / 30.3, 256 rows of 131071 - / 56.6 / 52.3 (so 512 and 1024 are
+// level from 10 to 17 million logits, and the border lies there).  At most 256 chunks.
 struct Chunks { int per, n; };
 Chunks chunks_of(uint64_t rows, uint32_t vocab) {
     const uint64_t logits = rows * vocab;
