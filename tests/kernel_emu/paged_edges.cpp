@@ -1,8 +1,6 @@
 // More of the paged-cache kernels' own source on the CPU, one check per name on the command line: how near the rotary positions
-// come to the formula.  (The buffers and pools are paged_cache.cpp's.)
-#define main paged_cache_main
-#include "paged_cache.cpp"
-#undef main
+// come to the formula.  (The buffers and pools are paged_cache.cpp's, its text up to the first check.)
+#include "paged_pool.inc"
 
 // Rotated fp32 queries and keys against long double.  Allowed for each: sine and cosine (with the magnitude) rounded to fp32 once,
 // two products and a sum, each half a step of 2^-24, and the angle's own rounding in 64 bits: a * 2^-53.

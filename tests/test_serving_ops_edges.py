@@ -23,6 +23,8 @@ def emulated(tmp_path_factory):
     for name in ("paged", "verify", "wave64"):
         text = open(os.path.join(ROOT, "rustane_amd", "csrc", "hipdec_%s.h" % name)).read()
         (build / ("kernel_%s.inc" % name)).write_text(re.sub(r"^#(pragma once|include .*)$", "", text, flags=re.M))
+    pool = open(os.path.join(EMU, "paged_cache.cpp")).read()
+    (build / "paged_pool.inc").write_text(pool[:pool.index("template <int HD")])
     built = {}
     # products and sums fused where the GPU's compiler fuses them, if this machine can
     fused = ["-mfma", "-ffp-contract=fast-honor-pragmas"] if re.search(r"^flags.* fma ", open("/proc/cpuinfo").read(), re.M) else []
