@@ -2419,6 +2419,7 @@ int hipdec_requests_admit(hipdec_model *m, uint32_t seq) {
     if (seq >= r.max_seqs || r.lens[seq] >= 0) return fail(m, HIPDEC_ERR_ARG, "sequence out of range or admitted already");
     if (request_pages_missing(m, seq, m->len) > r.free_pages.size()) return fail(m, HIPDEC_ERR_FULL, "not enough free pages");
     HCHK(hipSetDevice(m->opt.device));
+    (void)hipGetLastError();                                  // (an earlier call's, not this one's launches')
     HCHK(hipStreamSynchronize(m->stream));
     const RequestTrim trim{m, &seq, 1};
     request_pages(m, seq, m->len);
@@ -2490,6 +2491,7 @@ int hipdec_requests_step(hipdec_model *m, size_t n_seqs, const uint32_t *seqs, c
 
     const int R = (int)(n_seqs * S);
     HCHK(hipSetDevice(m->opt.device));
+    (void)hipGetLastError();                                    // (an earlier call's, not this one's launches')
     int rc = pf_ensure(m, R, true);
     if (rc) return rc;
     if (draft_probs && K && temperature > 0.0f && !r.d_probs && (rc = dalloc(m, &r.d_probs, (size_t)kRequestRows * c.vocab * 4))) return rc;

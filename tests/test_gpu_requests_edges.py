@@ -1,10 +1,13 @@
 """Requests stepped together (hipdec_requests_*) at the edge of what include/hip_decode.h allows."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 from rustane_amd import hipdec
 from rustane_amd.hipdec import HipDecodeError, KvDtype, NO_TOKEN
 from test_gpu_requests import admit, alone, close, model
+from test_zz_no_alloc import Hip
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +88,18 @@ def test_lengths_of_no_sequence_say_so():
         with pytest.raises(HipDecodeError) as e:
             m.requests_len(s)
         assert "no such sequence" in str(e.value)
+
+
+def test_an_error_that_the_program_left_is_not_a_step_s():
+    m, hip = model(), Hip()
+    m.requests_open(8, 8, 2)
+    m.set_len(0)
+    m.prefill(np.arange(9, dtype=np.uint32))
+    too_much = lambda: hip.rt.hipMalloc(C.byref(C.c_void_p()), 1 << 60)  # noqa: E731  (refused, and noted as the thread's last error)
+    assert too_much() != 0
+    m.requests_admit(1)
+    assert m.requests_len(1)[0] == 9
+    assert too_much() != 0
+    lg = m.requests_step([1], [3], logits=True)[2]
+    assert m.requests_len(1)[0] == 10
+    close(lg[0], alone(m, np.arange(9), [3]), 2e-3)
